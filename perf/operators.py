@@ -178,7 +178,7 @@ def _plan(st):
     fits = pages <= width
     need = torch.where(fits, (pages - owned).clamp(min=0), 0)
     upto = need.cumsum(0)
-    granted = fits & (upto <= st['n_free'])
+    granted = fits & ((need == 0) | (upto <= st['n_free']))
     kv = torch.where(granted, total, 0)
     owned_out = torch.where(granted, torch.maximum(owned, pages), owned)
     n_free = st['n_free'] - torch.where(granted, need, 0).sum()
