@@ -17,6 +17,21 @@ import torch.distributed as dist
 from .arena import ParamArena
 
 
+def _on_host(group):
+    """Does the group's backend want its tensors in host memory?  (gloo: its collectives on device tensors stage through pinned buffers of their own, which
+    several ranks on one device can exhaust, and have hung; the functional checks copy to the host and back instead, synchronously.)"""
+    return dist.is_initialized() and dist.get_backend(group) == 'gloo'
+
+
+def _broadcast(t, src, group=None):
+    if t.is_cuda and _on_host(group):
+        h = t.cpu()
+        dist.broadcast(h, src=src, group=group)
+        t.copy_(h)
+    else:
+        dist.broadcast(t, src=src, group=group)
+
+
 class GradReducer:
     def __init__(self, model, bucket_bytes=64 << 20, process_group=None, overlap=True, always=False, mode='all_reduce',
                  wire_dtype=torch.float32, tail_bytes=None, transport='torch', comm=None):
@@ -90,7 +105,7 @@ class GradReducer:
     def broadcast_parameters(model, src=0):
         """DDP constructor semantics: every rank starts from rank ``src``'s parameters (func/train.py:775-778)."""
         arena = model.arena
-        dist.broadcast(arena.master, src=src)
+        _broadcast(arena.master, src)
         arena.refresh_shadow(force=True)
 
     def broadcast_parameters_abi(self, src=0):
@@ -103,11 +118,11 @@ class GradReducer:
         """Every rank continues from rank ``src``'s momentum buffers (after steps in which the replicas were allowed to drift apart)."""
         buf = getattr(optimizer, 'momentum_buf', None)             # avt_amd.optim.FusedSGD: one flat buffer
         if torch.is_tensor(buf):
-            dist.broadcast(buf, src=src)
+            _broadcast(buf, src)
         for st in getattr(optimizer, 'state', {}).values():        # a torch optimizer: per-parameter state tensors
             for v in (st.values() if isinstance(st, dict) else ()):
                 if torch.is_tensor(v) and v.numel() > 1:
-                    dist.broadcast(v, src=src)
+                    _broadcast(v, src)
 
     def start_step(self):
         self._lo = self._sent = self.arena.total
@@ -182,6 +197,15 @@ class GradReducer:
             else:
                 self.comm.all_reduce(buf)
             return _Done()
+        if buf.is_cuda and _on_host(self.group):                # a copy in host memory, waited for (.cpu()), summed there, and back
+            host = buf.cpu()
+            self._collective(host).wait()
+            buf.copy_(host)
+            return _Done()
+        return self._collective(buf)
+
+    def _collective(self, buf):
+        n = buf.numel()
         if self.mode == 'rs_ag' and n % self.world == 0:
             # (bucket edges are multiples of 64 * world, so finish()'s bucket [0, lo) and every full bucket divide; the bucket that can fail
             #  to is the one whose upper end is the arena's end -- the first full bucket or the early-tail bucket [lo, total): the arena's size

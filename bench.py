@@ -300,13 +300,13 @@ def main(argv=None):
     # and each rank's device identity (N ranks on N distinct devices, or -- gloo functional check -- sharing some)
     ranks_seen, devices_seen = 1, None
     if dist_on:
-        one = torch.ones(1, device=device, dtype=torch.float32)
+        one = torch.ones(1, device=device if args.backend == 'nccl' else 'cpu', dtype=torch.float32)
         dist.all_reduce(one)
         ranks_seen = int(one.item())
         devices_seen = [None] * world
         pr = torch.cuda.get_device_properties(device)
         dist.all_gather_object(devices_seen, f'{pr.name} #{local} pci {getattr(pr, "pci_bus_id", "?")}:{getattr(pr, "pci_device_id", "?")}')
-    t = torch.tensor([elapsed_local], device=device, dtype=torch.float64)
+    t = torch.tensor([elapsed_local], device=device if args.backend == 'nccl' else 'cpu', dtype=torch.float64)
     per_rank = [t.clone() for _ in range(world)]
     if dist_on:
         dist.all_gather(per_rank, t)
