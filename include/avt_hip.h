@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define AVT_ABI_VERSION 9
+#define AVT_ABI_VERSION 10
 
 const char* avt_last_error(void);
 int avt_abi_version(void);
@@ -324,6 +324,39 @@ int avt_sgd_step(float* param, float* grad, float* momentum_buf, void* shadow_bf
  * Warm the library up on the capturing stream first (the persistent GEMM's ticket block of a new stream is allocated at its first launch). */
 int avt_sgd_step_dev(float* param, float* grad, float* momentum_buf, void* shadow_bf16, long n, const float* lr_dev, float momentum,
                      float weight_decay, float grad_scale, int nesterov, int first_step, int zero_grad, void* stream);
+
+/* ---- many streams on one paged key / value cache (ABI 10) ---------------------------------------------------------------
+ * What `past_key_values` is to one batch of clips of one length (models/future_prediction.py:168-202), for streams of different lengths that grow by
+ * chunks: a pool of pages of `page` tokens (a power of two in [8, 1024]), kcache / vcache bf16 [npages][page][Hkv][head_dim], and per stream a row of
+ * `width` page numbers in `table` (int32, row stride ldt).  All int32 arrays live on the device, so a step can be captured and replayed.
+ * avt_paged_plan: R <= 4096 streams of lens[r] cached tokens that own owned[r] pages each take fresh[r] >= 0 new tokens, packed one stream behind the
+ *   other into T token rows; free_pages[0 .. *n_free) (at most nfree_max) is a stack of free pages.
+ *     cu [R + 1]      first token row of each stream (running sum of fresh);  rows behind cu[R]: slot, position and stream -1
+ *     pages           stream r needs max(0, ceil((lens + fresh) / page) - owned) more, popped off the stack in the order of the streams and written behind
+ *                     the table's owned[r] entries.  A stream is refused when its pages pass `width`, its token rows pass T, or the stack does not hold what it and
+ *                     the streams in front of it need: it gets no page, kv_lens 0 (its rows see no key) and slots -1; a stream that needs none is never short.
+ *     kv_lens, owned_out [R], n_free_out [1]      what holds after the step;  slots [T] = page * `page` + offset, positions [T], streams [T]
+ *   The inputs are only read (but for the new table entries), so that the same call again gives the same result.
+ * avt_paged_kv_write: row t of k / v [T][width] (row strides ldk, ldv) goes to row slots[t] of both caches; slots outside [0, nslots) write nothing.
+ *   Slots are distinct (a plan's are): of two rows for one slot either may be found there.
+ * avt_paged_attn_fwd: q [T][H][head_dim] (token stride ldq), out [T][H * head_dim] (row stride ldo): rows cu[r] .. cu[r + 1) are the n newest of stream r's
+ *   kv_lens[r] cached tokens; row i of them sits at x = kv_lens[r] - n + i and out = softmax(scale q k[0..x]^T) v[0..x] with the kv head h / (H / Hkv); 0 where
+ *   no key is seen.  Keys a row does not see have no influence on it, whatever their bits.  A table entry outside [0, npages) names no page: its keys are not seen.
+ *   Rows behind cu[R] are left as they are.  head_dim % 8 == 0, <= 1024.  max_new / max_kv: what the caller knows of the longest chunk and of the longest
+ *   kv_lens (0: nothing); they choose kernels and grids, results hold for any lengths.  ws: avt_paged_attn_workspace_bytes of the same arguments.
+ * avt_w4_linear: y[m, n] = epilogue(sum_k x[m, k] s[n, k / group] (u[n, k] - 8)): x bf16 [M][K], u in 0 .. 15 two to a byte (q [N][K / 2], the low nibble holds
+ *   the even k), s bf16 [N][K / group], group 32 / 64 / 128; + bias (fp32), act 2: tanh GELU, + res (bf16); out_mode 0: bf16, 1: fp32. */
+int avt_paged_plan(const int* lens, const int* fresh, const int* owned, int* table, int ldt, int width, const int* free_pages, int nfree_max,
+                   const int* n_free, int page, int R, int T, int* cu, int* kv_lens, int* owned_out, int* n_free_out, int* slots, int* positions,
+                   int* streams, void* stream);
+int avt_paged_kv_write(const void* k, long ldk, const void* v, long ldv, void* kcache, void* vcache, const int* slots, long nslots, int T, int width,
+                       void* stream);
+int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, const void* vcache, long npages, int page, const int* table, int ldt, int width,
+                       const int* cu, const int* kv_lens, void* out, long ldo, int T, int R, int H, int Hkv, int head_dim, float scale,
+                       int max_new, int max_kv, void* ws, size_t ws_bytes, void* stream);
+size_t avt_paged_attn_workspace_bytes(int T, int R, int H, int Hkv, int head_dim, int max_new, int max_kv);
+int avt_w4_linear(const void* x, long ldx, const void* q, const void* scales, int group, const float* bias, int act, const void* res, long ldres,
+                  void* out, long ldo, int out_mode, int M, int N, int K, void* stream);
 
 /* ---- gradient exchange over RCCL (ABI 8) ------------------------------------------------------------------------------
  * What the reference gets from torch.nn.parallel.DistributedDataParallel(model, device_ids=[gpu]) (func/train.py:771-778) after
