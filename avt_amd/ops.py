@@ -792,7 +792,8 @@ def paged_attn(q, kcache, vcache, table, cu, kv_lens, *, scale=None, max_new=0, 
     _here(q, kcache, vcache, table, cu, kv_lens, out)
     if out is None:
         out = torch.empty((T, H * hd), device=q.device, dtype=BF16)
-    dims = (T, R, H, Hkv, hd, int(max_new), int(max_kv))
+    cap = table.size(1) * page
+    dims = (T, R, H, Hkv, hd, int(max_new), min(int(max_kv), cap) if max_kv > 0 else cap)
     ws = torch.empty(_lib.load().avt_paged_attn_workspace_bytes(*dims), device=q.device, dtype=torch.uint8)      # (its own: two captured steps share nothing)
     _lib.call('avt_paged_attn_fwd', _p(q), ldq, _p(kcache), _p(vcache), P, page, _p(table), _ld(table), table.size(1), _p(cu), _p(kv_lens), _p(out), _ld(out),
               *dims[:5], float(hd) ** -0.5 if scale is None else float(scale), *dims[5:], _p(ws), ws.numel(), _stream())
