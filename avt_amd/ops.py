@@ -4,6 +4,7 @@ Every function enqueues HIP kernels on torch's current stream and returns immedi
 GPU; there is no CPU or eager fallback -- a missing library raises ``AvtHipError``.
 """
 import bisect
+import functools
 
 import torch
 
@@ -707,25 +708,31 @@ def linear_softmax_xent_bwd(logits, target, lse, gloss, x, w, C, dw=None, dbias=
 I32 = torch.int32
 
 
-def _need(ok, msg):
-    if not ok:
-        raise _lib.AvtHipError(msg)
+def _refuse(msg):
+    raise _lib.AvtHipError(msg)
 
 
 def _here(first, *tensors):
-    """Every tensor on the current device: the kernels go to its current stream."""
+    """Every tensor on the current device: the kernels go to its current stream, which is returned."""
     dev = first.device
-    for t in (first,) + tensors:
+    for t in tensors:
         if t is not None and t.device != dev:
-            raise _lib.AvtHipError(f'tensors on different devices ({dev}, {t.device})')
+            _refuse(f'tensors on different devices ({dev}, {t.device})')
     if dev.type != 'cuda':
-        raise _lib.AvtHipError(f'tensors must live on a GPU, got {dev} (no CPU fallback exists)')
+        _refuse(f'tensors must live on a GPU, got {dev} (no CPU fallback exists)')
     if dev.index != torch.cuda.current_device():
-        raise _lib.AvtHipError(f'tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}')
+        _refuse(f'tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}')
+    return torch._C._cuda_getCurrentRawStream(dev.index)       # (the handle alone: torch.cuda.current_stream() builds an object around it, 2 us of a call of 10)
 
 
 def _ints(n, name, t):
-    _need(t.dtype == I32 and t.is_contiguous() and t.numel() == n, f'{name} must be {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}')
+    if t.dtype != I32 or t.numel() != n or not t.is_contiguous():
+        _refuse(f'{name} must be {n} contiguous int32 values, got {tuple(t.shape)} {t.dtype}')
+
+
+def _table_of(table, R):
+    if table.dtype != I32 or table.dim() != 2 or table.size(0) != R or table.size(1) < 1 or table.stride(1) != 1:
+        _refuse(f'table must be int32 [{R}, width] with unit inner stride, got {tuple(table.shape)} {table.dtype}')
 
 
 class PagedPlan:
@@ -737,32 +744,36 @@ def paged_plan(lens, new, owned, table, free, n_free, page, tokens):
     """Tables and slots of a step in which stream r's ``new[r]`` tokens join its ``lens[r]`` cached ones (avt_paged_plan): new pages are popped off
     ``free[:n_free]`` into ``table`` [R, width] behind the ``owned[r]`` a stream has; the tokens are packed into ``tokens`` rows.  A stream that cannot be served
     (pages past the table's width, rows past ``tokens``, not enough free pages) gets kv_lens 0 and slots -1.  Apart from the table the inputs stay as they are."""
-    R = lens.numel()
-    _ints(R, 'lens', lens); _ints(R, 'new', new); _ints(R, 'owned', owned); _ints(1, 'n_free', n_free); _ints(free.numel(), 'free', free)
-    _need(table.dtype == I32 and table.dim() == 2 and table.size(0) == R and table.size(1) > 0 and table.stride(1) == 1,
-          f'table must be int32 [{R}, width] with unit inner stride, got {tuple(table.shape)} {table.dtype}')
-    _here(lens, new, owned, table, free, n_free)
-    tokens = int(tokens)
-    buf = torch.empty(3 * R + 2 + 3 * max(tokens, 0), device=lens.device, dtype=I32)
+    R, F = lens.numel(), free.numel()
+    _ints(R, 'lens', lens); _ints(R, 'new', new); _ints(R, 'owned', owned); _ints(1, 'n_free', n_free); _ints(F, 'free', free)
+    _table_of(table, R)
+    stream = _here(lens, new, owned, table, free, n_free)
+    rows = max(int(tokens), 0)
+    buf = torch.empty(3 * R + 2 + 3 * rows, device=lens.device, dtype=I32)
     p = PagedPlan()
-    p.cu, p.kv_lens, p.owned, p.n_free, p.slots, p.positions, p.streams = buf.split([R + 1, R, R, 1] + 3 * [max(tokens, 0)])
+    p.cu, p.kv_lens, p.owned, p.n_free, p.slots, p.positions, p.streams = buf.split((R + 1, R, R, 1, rows, rows, rows))
     a = buf.data_ptr()
     b = a + 4 * (3 * R + 2)
-    _lib.call('avt_paged_plan', _p(lens), _p(new), _p(owned), _p(table), _ld(table), table.size(1), _p(free), free.numel(), _p(n_free), int(page), R, tokens,
-              a, a + 4 * (R + 1), a + 4 * (2 * R + 1), a + 4 * (3 * R + 1), b, b + 4 * tokens, b + 8 * tokens, _stream())
+    _lib.call('avt_paged_plan', lens.data_ptr(), new.data_ptr(), owned.data_ptr(), table.data_ptr(), _ld(table), table.size(1), free.data_ptr(), F, n_free.data_ptr(),
+              page, R, int(tokens), a, a + 4 * (R + 1), a + 4 * (2 * R + 1), a + 4 * (3 * R + 1), b, b + 4 * rows, b + 8 * rows, stream)
     return p
 
 
 def _cache_dims(kcache, vcache):
-    _need(kcache.dim() == 4 and kcache.shape == vcache.shape and kcache.is_contiguous() and vcache.is_contiguous() and kcache.dtype == vcache.dtype == BF16,
-          'the caches must be two contiguous bf16 tensors [pages, page, kv heads, head_dim]')
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or kcache.dtype != BF16 or vcache.dtype != BF16 or not kcache.is_contiguous() or not vcache.is_contiguous():
+        _refuse('the caches must be two contiguous bf16 tensors [pages, page, kv heads, head_dim]')
     return kcache.shape
 
 
 def _token_rows(t, name):
     """[T, heads, head_dim] bf16 with contiguous heads (a slice of a fused projection's rows): its token stride."""
-    _need(t.dim() == 3 and t.dtype == BF16 and t.stride(2) == 1 and (t.stride(1) == t.size(2) or t.size(1) == 1), f'{name} must be bf16 [tokens, heads, head_dim] with contiguous heads')
-    return t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2)
+    if t.dim() != 3 or t.dtype != BF16:
+        _refuse(f'{name} must be bf16 [tokens, heads, head_dim], got {tuple(t.shape)} {t.dtype}')
+    T, H, hd = t.shape
+    st, sh, sd = t.stride()
+    if sd != 1 or (sh != hd and H != 1):
+        _refuse(f'{name} must have contiguous heads, got strides {(st, sh, sd)}')
+    return st if T > 1 else H * hd
 
 
 def paged_kv_write(k, v, kcache, vcache, slots):
@@ -770,10 +781,16 @@ def paged_kv_write(k, v, kcache, vcache, slots):
     P, page, H, hd = _cache_dims(kcache, vcache)
     T = k.size(0)
     ldk, ldv = _token_rows(k, 'k'), _token_rows(v, 'v')
-    _need(tuple(k.shape) == tuple(v.shape) == (T, H, hd), f'k and v must be [{T}, {H}, {hd}] as the caches\' rows, got {tuple(k.shape)} and {tuple(v.shape)}')
+    if k.shape != v.shape or k.size(1) != H or k.size(2) != hd:
+        _refuse(f"k and v must be [{T}, {H}, {hd}] as the caches' rows, got {tuple(k.shape)} and {tuple(v.shape)}")
     _ints(T, 'slots', slots)
-    _here(k, v, kcache, vcache, slots)
-    _lib.call('avt_paged_kv_write', _p(k), ldk, _p(v), ldv, _p(kcache), _p(vcache), _p(slots), P * page, T, H * hd, _stream())
+    stream = _here(k, v, kcache, vcache, slots)
+    _lib.call('avt_paged_kv_write', k.data_ptr(), ldk, v.data_ptr(), ldv, kcache.data_ptr(), vcache.data_ptr(), slots.data_ptr(), P * page, T, H * hd, stream)
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_attn_workspace(*dims):
+    return _lib.load().avt_paged_attn_workspace_bytes(*dims)
 
 
 def paged_attn(q, kcache, vcache, table, cu, kv_lens, *, scale=None, max_new=0, max_kv=0, out=None):
@@ -781,22 +798,26 @@ def paged_attn(q, kcache, vcache, table, cu, kv_lens, *, scale=None, max_new=0, 
     (avt_paged_attn_fwd) -> [T, H * head_dim].  A chunk of one token is a decode step.  max_new / max_kv: the longest chunk and the longest kv_lens, as far as the caller
     knows them (they choose kernels, not results).  Rows behind cu[R] are not written."""
     P, page, Hkv, hd = _cache_dims(kcache, vcache)
-    T, H = q.size(0), q.size(1)
     ldq = _token_rows(q, 'q')
+    T, H, hq = q.shape
     R = kv_lens.numel()
-    _need(q.size(2) == hd and H % Hkv == 0, f'q must be [tokens, a multiple of {Hkv} heads, {hd}], got {tuple(q.shape)}')
+    if hq != hd or Hkv < 1 or H % Hkv:
+        _refuse(f'q must be [tokens, a multiple of {Hkv} heads, {hd}], got {tuple(q.shape)}')
     _ints(R, 'kv_lens', kv_lens); _ints(R + 1, 'cu', cu)
-    _need(table.dtype == I32 and table.dim() == 2 and table.size(0) == R and table.stride(1) == 1, f'table must be int32 [{R}, width] with unit inner stride, got {tuple(table.shape)} {table.dtype}')
-    if out is not None:
-        _need(out.dtype == BF16 and tuple(out.shape) == (T, H * hd) and out.stride(1) == 1, f'out must be bf16 [{T}, {H * hd}] with unit inner stride')
-    _here(q, kcache, vcache, table, cu, kv_lens, out)
+    _table_of(table, R)
+    stream = _here(q, kcache, vcache, table, cu, kv_lens, out)
     if out is None:
         out = torch.empty((T, H * hd), device=q.device, dtype=BF16)
-    cap = table.size(1) * page
+    elif out.dtype != BF16 or out.shape != (T, H * hd) or out.stride(1) != 1:
+        _refuse(f'out must be bf16 [{T}, {H * hd}] with unit inner stride')
+    width = table.size(1)
+    cap = width * page
     dims = (T, R, H, Hkv, hd, int(max_new), min(int(max_kv), cap) if max_kv > 0 else cap)
-    ws = torch.empty(_lib.load().avt_paged_attn_workspace_bytes(*dims), device=q.device, dtype=torch.uint8)      # (its own: two captured steps share nothing)
-    _lib.call('avt_paged_attn_fwd', _p(q), ldq, _p(kcache), _p(vcache), P, page, _p(table), _ld(table), table.size(1), _p(cu), _p(kv_lens), _p(out), _ld(out),
-              *dims[:5], float(hd) ** -0.5 if scale is None else float(scale), *dims[5:], _p(ws), ws.numel(), _stream())
+    need = _paged_attn_workspace(*dims)
+    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 16 else None           # (its own: two captured steps share nothing)
+    _lib.call('avt_paged_attn_fwd', q.data_ptr(), ldq, kcache.data_ptr(), vcache.data_ptr(), P, page, table.data_ptr(), _ld(table), width, cu.data_ptr(), kv_lens.data_ptr(),
+              out.data_ptr(), _ld(out), T, R, H, Hkv, hd, hd ** -0.5 if scale is None else float(scale), dims[5], dims[6], None if ws is None else ws.data_ptr(),
+              0 if ws is None else need, stream)
     return out
 
 
@@ -806,17 +827,19 @@ class W4Weight:
     __slots__ = ('q', 'scales', 'N', 'K', 'group')
 
     def __init__(self, q, scales):
-        _need(q.dim() == 2 and q.dtype == torch.uint8 and q.is_contiguous() and scales.dim() == 2 and scales.dtype == BF16 and scales.is_contiguous() and scales.size(0) == q.size(0),
-              'a 4-bit weight needs contiguous uint8 [N, K / 2] and bf16 [N, K / group]')
+        if q.dim() != 2 or q.dtype != torch.uint8 or not q.is_contiguous() or scales.dim() != 2 or scales.dtype != BF16 or not scales.is_contiguous() or scales.size(0) != q.size(0):
+            _refuse('a 4-bit weight needs contiguous uint8 [N, K / 2] and bf16 [N, K / group]')
         self.q, self.scales, self.N, self.K = q, scales, q.size(0), 2 * q.size(1)
         self.group = self.K // max(scales.size(1), 1)
-        _need(self.group in (32, 64, 128) and self.group * scales.size(1) == self.K, f'the group must be 32, 64 or 128 and divide K (K {self.K}, {scales.size(1)} groups)')
+        if self.group not in (32, 64, 128) or self.group * scales.size(1) != self.K:
+            _refuse(f'the group must be 32, 64 or 128 and divide K (K {self.K}, {scales.size(1)} groups)')
 
     @classmethod
     def quantize(cls, w, group=128):
         """w [N, K] (any float type) to the nearest 4-bit values of each group of k: scale = largest magnitude / 7 (rounded to bf16 first, so that the values
         are chosen for the scale that is stored), values -7 .. 7 about it."""
-        _need(w.dim() == 2 and group in (32, 64, 128) and w.size(1) % group == 0, f'w must be [N, K] with K a multiple of the group (32, 64 or 128), got {tuple(w.shape)}, {group}')
+        if w.dim() != 2 or group not in (32, 64, 128) or w.size(1) % group:
+            _refuse(f'w must be [N, K] with K a multiple of the group (32, 64 or 128), got {tuple(w.shape)}, {group}')
         g = w.detach().float().reshape(w.size(0), -1, group)
         s = (g.abs().amax(-1) / 7.0).to(BF16)
         sf = s.float()
@@ -831,19 +854,26 @@ class W4Weight:
 
 def w4_linear(x, w, *, bias=None, act=ACT_NONE, res=None, out_mode=OUT_BF16, out=None):
     """y[M, N] = epilogue(x[M, K] @ w^T) for a W4Weight (avt_w4_linear): + bias, tanh GELU, + res as in gemm(); made for few rows, where the weights' bytes count."""
+    N, K = w.N, w.K
+    if x.dim() != 2 or x.dtype != BF16 or x.size(1) != K or x.stride(1) != 1:
+        _refuse(f'x must be bf16 [M, {K}] with unit inner stride, got {tuple(x.shape)} {x.dtype}')
     M = x.size(0)
-    _need(x.dim() == 2 and x.dtype == BF16 and x.size(1) == w.K and x.stride(1) == 1, f'x must be bf16 [M, {w.K}] with unit inner stride, got {tuple(x.shape)} {x.dtype}')
-    _need(act in (ACT_NONE, ACT_GELU_TANH), 'act must be ACT_NONE or ACT_GELU_TANH')
-    _need(out_mode in (OUT_BF16, OUT_F32), 'out_mode must be OUT_BF16 or OUT_F32')
-    _need(bias is None or (bias.dtype == torch.float32 and bias.numel() == w.N and bias.is_contiguous()), f'bias must be {w.N} contiguous fp32 values')
-    _need(res is None or (res.dtype == BF16 and tuple(res.shape) == (M, w.N) and res.stride(1) == 1), f'res must be bf16 [{M}, {w.N}] with unit inner stride')
+    if act not in (ACT_NONE, ACT_GELU_TANH):
+        _refuse('act must be ACT_NONE or ACT_GELU_TANH')
+    if out_mode not in (OUT_BF16, OUT_F32):
+        _refuse('out_mode must be OUT_BF16 or OUT_F32')
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != N or not bias.is_contiguous()):
+        _refuse(f'bias must be {N} contiguous fp32 values')
+    if res is not None and (res.dtype != BF16 or res.shape != (M, N) or res.stride(1) != 1):
+        _refuse(f'res must be bf16 [{M}, {N}] with unit inner stride')
     dt = BF16 if out_mode == OUT_BF16 else torch.float32
-    _need(out is None or (out.dtype == dt and tuple(out.shape) == (M, w.N) and out.stride(1) == 1), f'out must be {dt} [{M}, {w.N}] with unit inner stride')
-    _here(x, w.q, w.scales, bias, res, out)
+    stream = _here(x, w.q, w.scales, bias, res, out)
     if out is None:
-        out = torch.empty((M, w.N), device=x.device, dtype=dt)
-    _lib.call('avt_w4_linear', _p(x), _ld(x), _p(w.q), _p(w.scales), w.group, _p(bias), act, _p(res), _ld(res) if res is not None else 0, _p(out), _ld(out),
-              out_mode, M, w.N, w.K, _stream())
+        out = torch.empty((M, N), device=x.device, dtype=dt)
+    elif out.dtype != dt or out.shape != (M, N) or out.stride(1) != 1:
+        _refuse(f'out must be {dt} [{M}, {N}] with unit inner stride')
+    _lib.call('avt_w4_linear', x.data_ptr(), _ld(x), w.q.data_ptr(), w.scales.data_ptr(), w.group, _p(bias), act, _p(res), 0 if res is None else _ld(res), out.data_ptr(), _ld(out),
+              out_mode, M, N, K, stream)
     return out
 
 
