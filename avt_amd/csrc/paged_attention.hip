@@ -377,8 +377,10 @@ template <int HD, int NQ, int BN>
 int launch_tiles(const AttnArgs& a, const Choice& c, hipStream_t st) {
   constexpr int lds = 4 * BN * HD * 2 + NQ * 4096 + 64;
   static_assert(lds <= 160 * 1024, "LDS");
-  const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_tile_kernel<HD, NQ, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  AVT_CHECK(e == hipSuccess, "avt_paged_attn_fwd: %s", hipGetErrorString(e));
+  if constexpr (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_tile_kernel<HD, NQ, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    AVT_CHECK(e == hipSuccess, "avt_paged_attn_fwd: %s", hipGetErrorString(e));
+  }
   hipLaunchKernelGGL((paged_attn_tile_kernel<HD, NQ, BN>), dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(256), lds, st, a);
   return 0;
 }

@@ -31,105 +31,158 @@ __device__ __forceinline__ void transpose4(u32x4_t& w) {
   w = (u32x4_t){c[0], d[0], c[1], d[1]};
 }
 
-// One workgroup (NW waves) per NT * 16 columns and up to MT * 16 rows; the waves take steps of 128 k in turn, and their sums meet in LDS, added in the order of
-// the waves.  A lane fetches 16 bytes of one row of weights (a step is 64 contiguous bytes of each of 16 rows), four words are exchanged between the lane groups so
-// that one product of the matrix unit covers 32 consecutive k, i.e. stays inside a group; products are of the exact integers 16 + u with the bf16 x, in fp32, and a
-// group ends with y += s (sum - 24 sum x): the weights are never rounded.  sum x comes from a product with ones, in the same layout.
-template <int MT, int NT, int GS, int NW>
-__global__ __launch_bounds__(NW * 64) void w4_linear_kernel(W4Args a) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  f32x4_t* part = (f32x4_t*)smem;                              // [NW][NT][MT][64 lanes]
+// One workgroup (8 waves) per NT * 16 columns and up to MT * 16 rows; the waves take steps of 128 k in turn, and their sums meet in LDS, added in the order of
+// the waves.  Products are of the exact integers 16 + u with the bf16 x, in fp32, and a group ends with y += s (sum - 24 sum x): the weights are never rounded.
+// sum x comes from a product with ones, in the same layout.
+//   A load whose neighbouring lanes read different rows takes the vector cache 4 cycles per 64 bytes (measured: 59 cycles for 64 x 16 bytes of 16 rows, and these
+// loads, not the bytes, set the time: 43 us of 33 x 16384 x 8192 against 24 without those of x), but that is how the matrix unit wants its operands.  So neighbouring
+// lanes fetch neighbouring bytes -- weights 64 bytes of each of 16 rows, copied straight into LDS, x 256 bytes of each of 4 rows, through registers -- and a wave
+// picks its fragments up from its own piece of LDS, where rows are swizzled over the banks; no wave waits for another before the end.  Four words of weights are then
+// exchanged between the lane groups, so that one product of the matrix unit covers 32 consecutive k, i.e. stays inside a group.
+template <int MT, int NT, int GS, int XE>
+__global__ __launch_bounds__(512) void w4_linear_kernel(W4Args a) {
+  constexpr int NW = 8, GPS = 4 / GS, WAVE = 2 * NT * 1024 + 4096;       // GPS: groups of a step; WAVE: bytes of a wave: two steps of weights, 16 rows of x
+  constexpr int SC = NT * GPS, SL = (SC + 3) / 4;              // scales of a step per column, loads for them: each lane group fetches another one
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  f32x4_t* part = (f32x4_t*)smem;                              // [NW][NT][MT][64 lanes], at the end
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * NT * 16, m0 = blockIdx.y * MT * 16;
+  char* wl = smem + wave * WAVE;
+  char* xl = wl + 2 * NT * 1024;
   const size_t rowb = (size_t)a.K / 2;
-  const int steps = (a.K + 127) / 128;
+  const int full = a.K / 128;
   const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-  constexpr int GPS = 4 / GS;                                  // groups of a step
-  const uint8_t* qp[NT];
-  const bf16_t* sp[NT];
+  // (addresses: a uniform base, which moves with the step, and 32-bit lane offsets)
+  const uint8_t* qb = a.q + (size_t)n0 * rowb;
+  const bf16_t* sb = a.s + (size_t)n0 * a.groups;
+  const bf16_t* xb = a.x + (size_t)m0 * a.ldx;
+  const int wrow = lane >> 2, wpiece = (lane & 3) ^ (lane >> 4);          // a lane copies piece `wpiece` of row `wrow`: piece p of row r is kept at p ^ (r >> 2)
+  uint32_t qo[NT], so[SL];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int n = min(n0 + j * 16 + c16, a.N - 1);             // (columns behind the last one repeat it and are not stored)
-    qp[j] = a.q + n * rowb + g * 16;
-    sp[j] = a.s + (size_t)n * a.groups;
-  }
-  const bf16_t* xp[MT];
-  bool live[MT];
+  for (int j = 0; j < NT; ++j) qo[j] = (uint32_t)min(j * 16 + wrow, a.N - 1 - n0) * (uint32_t)rowb;      // (columns behind the last one repeat it and are not stored)
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    live[i] = m0 + i * 16 + c16 < a.M;
-    xp[i] = a.x + (size_t)(live[i] ? m0 + i * 16 + c16 : m0) * a.ldx + g * 8;
-  }
+  for (int k = 0; k < SL; ++k) so[k] = (uint32_t)min(min(k * 4 + g, SC - 1) / GPS * 16 + c16, a.N - 1 - n0) * a.groups;
+  const int xrows = min(a.M - m0, MT * 16);
   f32x4_t y[NT][MT];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int i = 0; i < MT; ++i) y[j][i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
-  u32x4_t w[NT];
-  bf16_t sc[NT][GPS];
-  auto fetch = [&](int st) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      w[j] = (u32x4_t){0u, 0u, 0u, 0u};
-      if (st * 128 + g * 32 < a.K) w[j] = AVT_LDG_NT((const u32x4_t*)(qp[j] + (size_t)st * 64));
-#pragma unroll
-      for (int e = 0; e < GPS; ++e) sc[j][e] = sp[j][min(st * GPS + e, a.groups - 1)];
-    }
-  };
-  if (wave < steps) fetch(wave);
-  for (int st = wave; st < steps; st += NW) {
-    u32x4_t xv[MT][4];
+  u32x4_t xr[MT][XE];                                          // (XE = 1: at most 4 rows)
+  uint16_t sr[2][SL];
+  auto fetch_x = [&](int st, int live) {                       // live: 32-k pieces of the step that exist.  Load e of a tile: rows 4 e + g, 16 bytes per lane
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        xv[i][e] = (u32x4_t){0u, 0u, 0u, 0u};
-        if (live[i] && st * 128 + e * 32 < a.K) xv[i][e] = *(const u32x4_t*)(xp[i] + (size_t)st * 128 + e * 32);
+      for (int e = 0; e < XE; ++e)
+        xr[i][e] = *(const u32x4_t*)(xb + (size_t)st * 128 + ((uint32_t)min(i * 16 + e * 4 + g, xrows - 1) * (uint32_t)a.ldx + (c16 < live * 4 ? c16 : 0) * 8));
+  };
+  auto fetch_w = [&](int st, int d, int live) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(qb + (size_t)st * 64 + (qo[j] + (wpiece < live ? wpiece : 0) * 16)),
+                                       AVT_LDS_PTR(wl + (d * NT + j) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int k = 0; k < SL; ++k) sr[d][k] = sb[so[k] + min(st * GPS + min(k * 4 + g, SC - 1) % GPS, a.groups - 1)];
+  };
+  auto step = [&](int d, int live, auto&& next) {
+    u32x4_t w[NT];
+    bf16x8_t xf[MT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) w[j] = *(const u32x4_t*)(wl + (d * NT + j) * 1024 + c16 * 64 + ((g ^ (c16 >> 2)) << 4));
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int e = 0; e < XE; ++e) {                           // (written by hand: the compiler cannot tell these stores from the copies in flight, and waits for those)
+        const int row = e * 4 + g;
+        asm volatile("ds_write_b128 %0, %1" ::"v"(lds_addr32(xl) + row * 256 + ((c16 ^ row) << 4)), "v"(xr[i][e]) : "memory");
       }
-    u32x4_t cw[NT];
-    float cs[NT][GPS];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      cw[j] = w[j];
-#pragma unroll
-      for (int e = 0; e < GPS; ++e) cs[j][e] = bf2f(sc[j][e]);
+      for (int e = 0; e < 4; ++e) xf[i][e] = *(const bf16x8_t*)(xl + c16 * 256 + (((e * 4 + g) ^ c16) << 4));
     }
-    if (st + NW < steps) fetch(st + NW);
+    uint32_t sc[SL * 4];                                       // ... and to all four: scale q = (column tile, group of the step)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) transpose4(cw[j]);
+    for (int k = 0; k < SL; ++k) {
+      const uint32_t v = sr[d][k];
+      auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+      auto even = __builtin_amdgcn_permlane32_swap(p[0], p[0], false, false), odd = __builtin_amdgcn_permlane32_swap(p[1], p[1], false, false);
+      sc[k * 4] = even[0]; sc[k * 4 + 1] = odd[0]; sc[k * 4 + 2] = even[1]; sc[k * 4 + 3] = odd[1];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the fragments are in registers: the slot and xr are free
+    __builtin_amdgcn_sched_barrier(0);
+    next();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) transpose4(w[j]);
 #pragma unroll
     for (int e = 0; e < GPS; ++e) {
+      if (e * GS >= live) break;
       f32x4_t xs[MT];
-      bf16x8_t xf[MT][GS];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         xs[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int q = 0; q < GS; ++q) { xf[i][q] = pair8(xv[i][e * GS + q]); xs[i] = mfma16(xf[i][q], ones, xs[i]); }
+        for (int q = 0; q < GS; ++q) {
+          xf[i][e * GS + q] = pair8(__builtin_bit_cast(u32x4_t, xf[i][e * GS + q]));
+          xs[i] = mfma16(xf[i][e * GS + q], ones, xs[i]);
+        }
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         bf16x8_t wf[GS];
 #pragma unroll
-        for (int q = 0; q < GS; ++q) wf[q] = unpack8(cw[j][e * GS + q]);
+        for (int q = 0; q < GS; ++q) wf[q] = unpack8(w[j][e * GS + q]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int q = 0; q < GS; ++q) acc = mfma16(xf[i][q], wf[q], acc);
+          for (int q = 0; q < GS; ++q) acc = mfma16(xf[i][e * GS + q], wf[q], acc);
+          const float s = __uint_as_float(sc[j * GPS + e] << 16);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[j][i][r] = fmaf(cs[j][e], fmaf(-24.f, xs[i][r], acc[r]), y[j][i][r]);
+          for (int r = 0; r < 4; ++r) y[j][i][r] = fmaf(s, fmaf(-24.f, xs[i][r], acc[r]), y[j][i][r]);
         }
       }
     }
+  };
+  // The order of the requests is x (s + 1), weights (s + 2), and loads come back in order: when x (s) is there, so are the weights of s, and those of s + 1 may still
+  // be out.  Requests behind the last step repeat it (a conditional one makes the compiler copy what it loaded, i.e. wait for it).
+  const int mine = wave < full ? (full - wave + NW - 1) / NW : 0;
+  auto at = [&](int i) { return wave + min(i, mine - 1) * NW; };
+  if (mine > 0) {
+    fetch_w(at(0), 0, 4);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_x(at(0), 4);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_w(at(1), 1, 4);
+    auto turn = [&](int i, int d) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NT + SL) : "memory");
+      step(d, 4, [&] {
+        fetch_x(at(i + 1), 4);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_w(at(i + 2), d, 4);
+      });
+    };
+    int i = 0;
+    for (; i + 2 <= mine; i += 2) { turn(i, 0); turn(i + 1, 1); }
+    if (i < mine) turn(i, 0);
   }
+  if (a.K % 128 && wave == NW - 1) {                           // a last step of 32, 64 or 96 k
+    const int live = (a.K - full * 128) / 32;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    fetch_w(full, 0, live);
+    fetch_x(full, live);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    step(0, live, [] {});
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (the requests behind the last step still write into LDS)
+  __syncthreads();
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int i = 0; i < MT; ++i) part[((wave * NT + j) * MT + i) * 64 + lane] = y[j][i];
   __syncthreads();
-  for (int o = tid; o < NT * MT * 64; o += NW * 64) {
+  for (int o = tid; o < NT * MT * 64; o += 512) {
     f32x4_t v = part[o];
     for (int z = 1; z < NW; ++z) v += part[z * NT * MT * 64 + o];
     const int ln = o & 63, i = (o >> 6) % MT, j = (o >> 6) / MT;
@@ -149,21 +202,28 @@ __global__ __launch_bounds__(NW * 64) void w4_linear_kernel(W4Args a) {
   }
 }
 
-template <int MT, int NT, int GS, int NW>
+template <int MT, int NT, int GS, int XE>
 int launch(const W4Args& a, hipStream_t st) {
-  constexpr int lds = NW * NT * MT * 1024;
+  constexpr int ring = 8 * (2 * NT * 1024 + 4096), sums = 8 * NT * MT * 1024, lds = ring > sums ? ring : sums;
   static_assert(lds <= 160 * 1024, "LDS");
-  const hipError_t e = hipFuncSetAttribute((const void*)w4_linear_kernel<MT, NT, GS, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  AVT_CHECK(e == hipSuccess, "avt_w4_linear: %s", hipGetErrorString(e));
-  hipLaunchKernelGGL((w4_linear_kernel<MT, NT, GS, NW>), dim3((a.N + NT * 16 - 1) / (NT * 16), (a.M + MT * 16 - 1) / (MT * 16)), dim3(NW * 64), lds, st, a);
+  if constexpr (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)w4_linear_kernel<MT, NT, GS, XE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    AVT_CHECK(e == hipSuccess, "avt_w4_linear: %s", hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL((w4_linear_kernel<MT, NT, GS, XE>), dim3((a.N + NT * 16 - 1) / (NT * 16), (a.M + MT * 16 - 1) / (MT * 16)), dim3(512), lds, st, a);
   return 0;
+}
+template <int NT, int GS>
+int launch_cols(const W4Args& a, hipStream_t st) {
+  if (a.M <= 4) return launch<1, NT, GS, 1>(a, st);
+  if (a.M <= 16) return launch<1, NT, GS, 4>(a, st);
+  if (a.M <= 32) return launch<2, NT, GS, 4>(a, st);
+  if (a.M <= 48) return launch<3, NT, GS, 4>(a, st);
+  return launch<4, NT < 4 ? NT : 2, GS, 4>(a, st);             // (4 x 4 tiles do not fit the registers)
 }
 template <int GS>
 int launch_rows(const W4Args& a, hipStream_t st) {
-  const bool wide = a.N >= 64 * 192;                           // enough workgroups of 64 columns for most of the CUs
-  const int mt = a.M > 48 ? 4 : (a.M + 15) / 16;
-  if (wide) return mt == 1 ? launch<1, 4, GS, 8>(a, st) : mt == 2 ? launch<2, 4, GS, 8>(a, st) : mt == 3 ? launch<3, 4, GS, 8>(a, st) : launch<4, 4, GS, 8>(a, st);
-  return mt == 1 ? launch<1, 1, GS, 16>(a, st) : mt == 2 ? launch<2, 1, GS, 16>(a, st) : mt == 3 ? launch<3, 1, GS, 8>(a, st) : launch<4, 1, GS, 8>(a, st);
+  return a.N >= 64 * 192 ? launch_cols<4, GS>(a, st) : a.N >= 32 * 192 ? launch_cols<2, GS>(a, st) : launch_cols<1, GS>(a, st);
 }
 }  // namespace
 
@@ -179,6 +239,7 @@ extern "C" int avt_w4_linear(const void* x, long ldx, const void* q, const void*
   AVT_CHECK(ldx >= K && ldx % 8 == 0 && aligned16(x) && aligned16(q), "avt_w4_linear: 16-byte aligned rows of x and q required");
   AVT_CHECK(ldo >= N && (!res || ldres >= N), "avt_w4_linear: leading dimension below N");
   AVT_CHECK((M + 63) / 64 <= 65535, "avt_w4_linear: too many rows (%d)", M);
+  AVT_CHECK(K < (1 << 24) && ldx < (1 << 24), "avt_w4_linear: K and ldx below 2^24 (K %d, ldx %ld)", K, ldx);
   W4Args a;
   a.x = (const bf16_t*)x; a.q = (const uint8_t*)q; a.s = (const bf16_t*)scales; a.bias = bias; a.res = (const bf16_t*)res; a.out = out;
   a.ldx = ldx; a.ldres = ldres; a.ldo = ldo; a.M = M; a.N = N; a.K = K; a.groups = K / group; a.act = act; a.out_f32 = out_mode;
