@@ -31,6 +31,12 @@ __device__ __forceinline__ void transpose4(u32x4_t& w) {
   w = (u32x4_t){c[0], d[0], c[1], d[1]};
 }
 
+// 16 bytes per lane from base + voff + soff straight into LDS (lane l at lds + 16 l)
+__device__ __forceinline__ void copy_to_lds(const void* base, char* lds, uint32_t voff, uint32_t soff) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7FFFFFF0u, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, AVT_LDS_PTR(lds), 16, voff, soff, 0, 0);
+}
+
 // One workgroup (8 waves) per NT * 16 columns and up to MT * 16 rows; the waves take steps of 128 k in turn, and their sums meet in LDS, added in the order of
 // the waves.  Products are of the exact integers 16 + u with the bf16 x, in fp32, and a group ends with y += s (sum - 24 sum x): the weights are never rounded.
 // sum x comes from a product with ones, in the same layout.
@@ -81,8 +87,7 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4Args a) {
   auto fetch_w = [&](int st, int d, int live) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(qb + (size_t)st * 64 + (qo[j] + (wpiece < live ? wpiece : 0) * 16)),
-                                       AVT_LDS_PTR(wl + (d * NT + j) * 1024), 16, 0, 0);
+      copy_to_lds(qb, wl + (d * NT + j) * 1024, qo[j] + (wpiece < live ? wpiece : 0) * 16, st * 64);
 #pragma unroll
     for (int k = 0; k < SL; ++k) sr[d][k] = sb[so[k] + min(st * GPS + min(k * 4 + g, SC - 1) % GPS, a.groups - 1)];
   };
@@ -217,9 +222,8 @@ template <int NT, int GS>
 int launch_cols(const W4Args& a, hipStream_t st) {
   if (a.M <= 4) return launch<1, NT, GS, 1>(a, st);
   if (a.M <= 16) return launch<1, NT, GS, 4>(a, st);
-  if (a.M <= 32) return launch<2, NT, GS, 4>(a, st);
-  if (a.M <= 48) return launch<3, NT, GS, 4>(a, st);
-  return launch<4, NT < 4 ? NT : 2, GS, 4>(a, st);             // (4 x 4 tiles do not fit the registers)
+  if (a.M > 32 && a.M <= 48) return launch<3, (GS < 4 && NT > 2) ? 2 : NT, GS, 4>(a, st);      // (3 x 4 tiles of small groups do not fit the registers)
+  return launch<2, NT, GS, 4>(a, st);
 }
 template <int GS>
 int launch_rows(const W4Args& a, hipStream_t st) {
