@@ -22,14 +22,13 @@ __device__ __forceinline__ int find_stream(const int* __restrict__ cu, int R, in
   return cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
 }
 
-__device__ const u32x4_t ZERO_CHUNK = {0u, 0u, 0u, 0u};       // what a lane copies where there is no key (behind the last one, no page) or no column
-
 struct AttnArgs {
   const bf16_t* q; const bf16_t* kc; const bf16_t* vc; const int* table; const int* cu; const int* kv_lens;
   bf16_t* out; float* part_o; float* part_ml;                  // part_*: one partial result per split and row ([split][T * H][hd], [split][T * H] (max, sum))
   long ldq, ldo, npages;
   int shift, ldt, width, T, R, H, Hkv, grp, hd, nsplit, cmin;
-  float scale_log2;                                            // scale * log2(e): exponentials are powers of two
+  float scale_log2;                                            // |scale| log2(e): exponentials are powers of two
+  uint32_t q_and, q_xor;                                       // applied to q as it is read: the sign of a negative scale; a scale of 0 is a q of 0
 };
 
 // Keys of one split: a stream's cached tokens are cut into at most nsplit pieces, each a multiple of `cmin` keys (itself a multiple of the tile's).
@@ -38,16 +37,24 @@ __device__ __forceinline__ long split_keys(int kv, int nsplit, int cmin) {
   return (c + cmin - 1) / cmin * cmin;
 }
 
-// 16-byte piece c of row r of a [keys][HD] tile is kept at c ^ tile_swz(r): a copy into LDS fills whole rows lane by lane, so the swizzle is applied to what a lane
-// fetches.  8 consecutive rows land on 8 different 32-byte slots (transposing reads of V: 8 rows x 32 bytes per half wave), 16 rows on 16 different 16-byte slots
-// (row fragments of K); rows of 128 bytes pair up in a 256-byte line (the permutation of vit_attention.hip).
+typedef const __attribute__((address_space(4))) int* table_t;  // (the table does not change while a kernel runs: its entries come through the scalar cache)
+
+// 16-byte piece c of row r of a [keys][HD] tile is kept at c ^ swz(r): a copy into LDS fills whole rows lane by lane, so the swizzle is applied to what a lane
+// fetches.  Row fragments of K want 16 rows on 16 different 16-byte slots; the transposing reads of V take 8 rows x 32 bytes per half wave (16-row products) or
+// 4 rows x 64 bytes (32-row products), which want 8 rows on 8 different 32-byte slots or 4 rows on 4 different 64-byte ones.  Rows of 128 bytes pair up in a line.
 template <int HD>
-__device__ __forceinline__ int tile_swz(int r) {
+__device__ __forceinline__ int swz16(int r) {
   if constexpr (HD == 64) { const int p = (r >> 1) & 7, hi = p >> 2; return (((p & 3) ^ (hi << 1)) << 1) | hi; }
   else return ((r & 7) << 1) | ((r >> 3) & 1);
 }
+template <int HD>
+__device__ __forceinline__ int swz32(int r) {
+  if constexpr (HD == 64) { const int p = (r >> 1) & 7; return ((p & 1) << 2) | (p >> 1); }
+  else return ((r & 3) << 2) | ((r >> 2) & 3);
+}
 
 __device__ __forceinline__ f32x4_t mfma16(bf16x8_t a, bf16x8_t b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float gsum(float v) { v += __shfl_xor(v, 16, 64); return v + __shfl_xor(v, 32, 64); }
 __device__ __forceinline__ float gmax(float v) { v = fmaxf(v, __shfl_xor(v, 16, 64)); return fmaxf(v, __shfl_xor(v, 32, 64)); }
 
@@ -66,81 +73,161 @@ __device__ __forceinline__ int find_tile(const int* __restrict__ cu, int R, int 
   return lo;
 }
 
-// One workgroup (4 waves) per (kv head, tile of NQ * 16 rows, split of the keys).  K and V tiles of BN keys come into LDS by direct copies, row by row through the
-// page table, two tiles in turn.  S^T = K Q^T: wave w takes 16 keys (w % KT) of the tile and, where the tile has fewer than 64 keys, its share of the head's
+__device__ __forceinline__ u32x4_t read_q(const AttnArgs& a, const bf16_t* p) {
+  u32x4_t v = *(const u32x4_t*)p;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (v[e] & a.q_and) ^ a.q_xor;
+  return v;
+}
+
+// What a workgroup works on: rows row0 .. of a stream's `rows`, keys k0 .. k1 - 1.
+struct Work {
+  int hk, sp, t0, n, row0, rows, kv, k0, k1;
+  bool gap;                                                    // some table entry of the range names no page
+  table_t tab;
+};
+__device__ __forceinline__ int row_pos(const Work& w, int row, int grp) { return w.kv - w.n + row / grp; }
+__device__ __forceinline__ bool find_work(const AttnArgs& a, int bm, int lane, Work& w) {
+  w.hk = blockIdx.x % a.Hkv;
+  w.sp = blockIdx.y;
+  const int tile = (gridDim.x - 1 - blockIdx.x) / a.Hkv;       // (the last rows of a chunk see the most keys: first)
+  const int r = __builtin_amdgcn_readfirstlane(find_tile(a.cu, a.R, a.T, a.grp, bm, tile, lane));
+  w.t0 = max(0, min(a.cu[r], a.T));
+  w.n = max(0, min(a.cu[r + 1], a.T) - w.t0);
+  w.row0 = (tile - tile_base(a.cu, r, a.T, a.grp, bm)) * bm;
+  w.rows = w.n * a.grp;
+  if (w.row0 < 0 || w.row0 >= w.rows) return false;
+  w.kv = (int)min((long)max(a.kv_lens[r], 0), (long)a.width << a.shift);
+  const int last = row_pos(w, min(w.row0 + bm, w.rows) - 1, a.grp);
+  const long chunk = split_keys(w.kv, a.nsplit, a.cmin);
+  w.k0 = (int)min((long)w.sp * chunk, (long)w.kv);
+  w.k1 = (int)min((long)(w.sp + 1) * chunk, (long)(last + 1));
+  if (w.k0 >= w.k1 && a.nsplit > 1) return false;              // (the join knows)
+  w.tab = (table_t)(a.table + (size_t)r * a.ldt);
+  bool gap = false;
+  if (w.k0 < w.k1)
+    for (int e = (w.k0 >> a.shift) + lane; e <= (w.k1 - 1) >> a.shift; e += 64) { const int pg = a.table[(size_t)r * a.ldt + e]; gap |= pg < 0 || pg >= a.npages; }
+  w.gap = __any(gap);
+  return true;
+}
+
+// Copies of K and V tiles of BN keys into LDS by 4 waves, 1 KB an instruction: its rows lie in one page (a page holds at least 8 tokens), so the page's address is
+// scalar and a lane's offset within it does not change from tile to tile.  Rows behind the last key, rows of no page and columns behind the head's are asked for
+// out of range and arrive as zeros: what is not finite in memory that holds no key never meets a probability of 0.
+template <int HD, int BN, int (*SWZ)(int)>
+struct Copier {
+  static constexpr int ROWB = HD * 2, TILEB = BN * ROWB, NI = TILEB / 4096;
+  static constexpr uint32_t NONE = 0xFFFFFFF0u;
+  uint32_t off[NI];
+  int pg[NI];
+  __device__ __forceinline__ void init(const AttnArgs& a, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int at = (i * 4 + wave) * 1024 + lane * 16, row = at / ROWB, c = ((at % ROWB) >> 4) ^ SWZ(row);
+      off[i] = c * 8 < a.hd ? (uint32_t)(((row - (i * 4 + wave) * 1024 / ROWB) * a.Hkv * a.hd + c * 8) * 2) : NONE;
+    }
+  }
+  __device__ __forceinline__ void pages(const AttnArgs& a, const Work& w, int j0, int wave) {      // of the tile that is issued next
+    if (j0 < w.k1) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) pg[i] = w.tab[min(j0 + (i * 4 + wave) * 1024 / ROWB, w.k1 - 1) >> a.shift];
+    }
+  }
+  __device__ __forceinline__ void issue(const AttnArgs& a, const Work& w, int j0, char* dst, int wave, int lane) {
+    const bool whole = j0 + BN <= w.k1 && !w.gap;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int jb = j0 + (i * 4 + wave) * 1024 / ROWB;
+      uint32_t v = off[i];
+      if (!whole) {
+        const int row = ((i * 4 + wave) * 1024 + lane * 16) / ROWB;
+        if (j0 + row >= w.k1 || pg[i] < 0 || pg[i] >= a.npages) v = NONE;
+      }
+      const size_t at = ((((size_t)(uint32_t)pg[i] << a.shift) + (jb & ((1 << a.shift) - 1))) * a.Hkv + w.hk) * a.hd;
+      copy(a.kc + at, dst + (i * 4 + wave) * 1024, v);
+      copy(a.vc + at, dst + TILEB + (i * 4 + wave) * 1024, v);
+    }
+  }
+  __device__ __forceinline__ static void copy(const bf16_t* base, char* lds, uint32_t voff) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7FFFFFF0u, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, AVT_LDS_PTR(lds), 16, voff, 0, 0, 0);
+  }
+};
+
+// A V fragment of a tile that some row sees a part of: values that are not finite are taken out (their rows' probabilities may be 0) and told from `code`, which is
+// 1 for a NaN, 2^8 for +inf and 2^16 for -inf: its product with the rows' visibility counts, exactly, what each row sees of them.
+__device__ __forceinline__ bool not_finite(bf16x8_t f) {
+  const u32x4_t w = __builtin_bit_cast(u32x4_t, f);
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+__device__ __forceinline__ void take_out(bf16x8_t& f, bf16x8_t& code) {
+  u32x4_t w = __builtin_bit_cast(u32x4_t, f), k = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int sh = (e & 1) * 16;
+    const uint32_t v = (w[e >> 1] >> sh) & 0xffffu;
+    if ((v & 0x7f80u) == 0x7f80u) {
+      w[e >> 1] &= ~(0xffffu << sh);
+      k[e >> 1] |= ((v & 0x7fu) ? 0x3f80u : (v & 0x8000u) ? 0x4780u : 0x4380u) << sh;
+    }
+  }
+  f = __builtin_bit_cast(bf16x8_t, w);
+  code = __builtin_bit_cast(bf16x8_t, k);
+}
+__device__ __forceinline__ float put_back(float o, float count) {
+  const int c = (int)count;
+  if (c & 0xff) o += NAN;
+  if (c & 0xff00) o += INFINITY;
+  if (c >> 16) o -= INFINITY;
+  return o;
+}
+__device__ __forceinline__ bf16x8_t seen8(uint32_t bits) {     // 8 bits -> 1.0 / 0.0
+  u32x4_t w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = ((bits >> (2 * e)) & 1u ? 0x3f80u : 0u) | ((bits >> (2 * e + 1)) & 1u ? 0x3f800000u : 0u);
+  return __builtin_bit_cast(bf16x8_t, w);
+}
+__device__ __forceinline__ bool page_there(const AttnArgs& a, const Work& w, int j) {
+  if (!w.gap || j >= w.k1) return true;
+  const int e = w.tab[j >> a.shift];
+  return e >= 0 && e < a.npages;
+}
+
+// ---- few rows: one workgroup (4 waves) per (kv head, tile of NQ * 16 rows, split of the keys) ------------------------------------------------------------------
+// K and V tiles of BN keys, two in turn.  S^T = K Q^T: wave w takes 16 keys (w % KT) of the tile and, where the tile has fewer than 64 keys, its share of the head's
 // columns (w / KT); the scores pass through LDS (16 bytes per lane, the same lane reads them) and every wave then has all of them in the layout of P^T, the right
 // operand of O^T = V^T P^T, and keeps the running maximum and sum (fp32) of every row for itself: no reduction between waves.  Wave w owns a quarter of the head's
 // columns of O.  P is rounded to bf16 for the product (the matrix unit's type; half a step 2^-8 of each probability), the sum is of the unrounded ones.
 template <int HD, int NQ, int BN>
 __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
   constexpr int ROWB = HD * 2, TILEB = BN * ROWB, KT = BN / 16, KS = 4 / KT, DS = HD / KS / 32, DT = HD / 64, TT = BN >= 32 ? BN / 32 : 1, BM = NQ * 16;
-  constexpr int NI = TILEB / 4096;                             // copies of 1 KB per wave and tensor
-  static_assert(KT * KS == 4 && DS >= 1 && NI >= 1 && 48 * ROWB < 65536 + 32 * ROWB, "tile shape");
-  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V], scores, flag
+  static_assert(KT * KS == 4 && DS >= 1 && TILEB >= 4096, "tile shape");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V], scores
   f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [NQ][4 waves][64 lanes]
-  int* odd = (int*)(smem + 4 * TILEB + NQ * 4096);             // some value of V in a partly hidden tile is not finite
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.x % a.Hkv, tile = (gridDim.x - 1 - blockIdx.x) / a.Hkv, sp = blockIdx.y;      // (the last rows of a chunk see the most keys: first)
-  const int r = __builtin_amdgcn_readfirstlane(find_tile(a.cu, a.R, a.T, a.grp, BM, tile, lane));
-  const int t0 = max(0, min(a.cu[r], a.T)), n = max(0, min(a.cu[r + 1], a.T) - t0);
-  const int row0 = (tile - tile_base(a.cu, r, a.T, a.grp, BM)) * BM, rows = n * a.grp;
-  if (row0 < 0 || row0 >= rows) return;
-  const int kv = (int)min((long)max(a.kv_lens[r], 0), (long)a.width << a.shift);
-  const int first = kv - n + row0 / a.grp, last = kv - n + (min(row0 + BM, rows) - 1) / a.grp;      // positions of the tile's first and last row
-  const long chunk = split_keys(kv, a.nsplit, a.cmin);
-  const int k0 = (int)min((long)sp * chunk, (long)kv), k1 = (int)min((long)(sp + 1) * chunk, (long)(last + 1));
-  if (k0 >= k1 && a.nsplit > 1) return;                        // (the join knows)
-  const int* tab = a.table + (size_t)r * a.ldt;
-  const int pmask = (1 << a.shift) - 1;
+  Work w;
+  if (!find_work(a, BM, lane, w)) return;
+  const int first = row_pos(w, w.row0, a.grp), last = row_pos(w, min(w.row0 + BM, w.rows) - 1, a.grp);
 
   int pos[NQ];                                                 // this lane's row (column of S^T): its position, -1: no row
   bf16x8_t qf[NQ][DS];
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
-    const int row = row0 + i * 16 + c16, tok = row / a.grp;
-    const bool ok = row < rows;
-    pos[i] = ok ? kv - n + tok : -1;
-    const bf16_t* p = a.q + (size_t)(t0 + (ok ? tok : 0)) * a.ldq + (size_t)(hk * a.grp + (ok ? row - tok * a.grp : 0)) * a.hd;
+    const int row = w.row0 + i * 16 + c16, tok = row / a.grp;
+    const bool ok = row < w.rows;
+    pos[i] = ok ? w.kv - w.n + tok : -1;
+    const bf16_t* p = a.q + (size_t)(w.t0 + (ok ? tok : 0)) * a.ldq + (size_t)(w.hk * a.grp + (ok ? row - tok * a.grp : 0)) * a.hd;
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       const int d = (wave / KT) * (HD / KS) + s * 32 + g * 8;
-      u32x4_t w = {0u, 0u, 0u, 0u};
-      if (ok && d < a.hd) w = *(const u32x4_t*)(p + d);
-      qf[i][s] = __builtin_bit_cast(bf16x8_t, w);
+      u32x4_t v = {0u, 0u, 0u, 0u};
+      if (ok && d < a.hd) v = read_q(a, p + d);
+      qf[i][s] = __builtin_bit_cast(bf16x8_t, v);
     }
   }
-  bool gap = false;                                            // a table entry of this range names no page
-  if (k0 < k1)
-    for (int e = (k0 >> a.shift) + lane; e <= (k1 - 1) >> a.shift; e += 64) { const int pg = tab[e]; gap |= pg < 0 || pg >= a.npages; }
-  gap = __any(gap);
-  if (tid == 0) *odd = 0;
-
-  // copies of one tile: instruction ii of the tile fills bytes [1024 ii, 1024 ii + 1024); its rows lie in one page (a page holds at least 8 tokens)
-  auto page_of = [&](int j0, int i) {
-    const int jb = j0 + (i * 4 + wave) * 1024 / ROWB;
-    return tab[min(jb, k1 - 1) >> a.shift];
-  };
-  int pg[NI];
-  auto issue = [&](int j0, int stage) {
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int at = (i * 4 + wave) * 1024 + lane * 16, row = at / ROWB, c = ((at % ROWB) >> 4) ^ tile_swz<HD>(row), j = j0 + row;
-      const bool ok = j < k1 && pg[i] >= 0 && pg[i] < a.npages && c * 8 < a.hd;
-      const size_t off = ((((size_t)(uint32_t)pg[i] << a.shift) + (j & pmask)) * a.Hkv + hk) * a.hd + c * 8;
-      const bf16_t* ks = ok ? a.kc + off : (const bf16_t*)&ZERO_CHUNK;
-      const bf16_t* vs = ok ? a.vc + off : (const bf16_t*)&ZERO_CHUNK;
-      char* dst = smem + stage * 2 * TILEB + (i * 4 + wave) * 1024;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)ks, AVT_LDS_PTR(dst), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vs, AVT_LDS_PTR(dst + TILEB), 16, 0, 0);
-    }
-  };
-  auto pages = [&](int j0) {
-    if (j0 < k1) {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) pg[i] = page_of(j0, i);
-    }
-  };
-
   f32x4_t o[NQ][DT];
   float m[NQ], l[NQ];
 #pragma unroll
@@ -149,21 +236,23 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[i][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
-  const int kswz = tile_swz<HD>(c16);
+  const int kswz = swz16<HD>(c16);
   const int krow = ((wave % KT) * 16 + c16) * ROWB, kc0 = (wave / KT) * (HD / KS / 8) + g;
   const int vr = 4 * g + (c16 >> 2);
-  const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((wave * (HD / 32) + ((c16 & 3) >> 1)) ^ tile_swz<HD>(vr)) << 4) + (c16 & 1) * 8;
+  const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((wave * (HD / 32) + ((c16 & 3) >> 1)) ^ swz16<HD>(vr)) << 4) + (c16 & 1) * 8;
 
   // (Q is waited for here: left to the first product, the compiler's wait for it would sit inside the loop and wait for the copies in flight as well)
 #pragma unroll
   for (int i = 0; i < NQ; ++i)
 #pragma unroll
     for (int s = 0; s < DS; ++s) asm volatile("" : "+v"(qf[i][s]));
-  if (k0 < k1) { pages(k0); issue(k0, 0); pages(k0 + BN); }
+  Copier<HD, BN, swz16<HD>> cp;
+  cp.init(a, wave, lane);
+  if (w.k0 < w.k1) { cp.pages(a, w, w.k0, wave); cp.issue(a, w, w.k0, smem, wave, lane); cp.pages(a, w, w.k0 + BN, wave); }
   int stage = 0;
-  for (int j0 = k0; j0 < k1; j0 += BN, stage ^= 1) {
+  for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one and with the scores
-    if (j0 + BN < k1) { issue(j0 + BN, stage ^ 1); pages(j0 + 2 * BN); }
+    if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
     const char* kt = smem + stage * 2 * TILEB;
     f32x4_t s4[NQ];
 #pragma unroll
@@ -176,19 +265,9 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) sx[(i * 4 + wave) * 64 + lane] = s4[i];
-    const bool hide = gap || j0 + BN - 1 > first;              // some row does not see some key of this tile
-    const bool uneven = first < last && j0 + BN - 1 > first;   // ... and another one does: a value that is not finite must not pass
-    if (uneven) {
-      bool bad = false;
-      for (int i = tid; i < TILEB / 16; i += 256) {
-        const u32x4_t w = *(const u32x4_t*)(kt + TILEB + i * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
-      }
-      if (__any(bad) && lane == 0) *odd = 1;
-    }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const bool slow = uneven && *odd;
+    const bool hide = w.gap || j0 + BN - 1 > first;            // some row does not see some key of this tile
+    uint32_t seen[NQ];
     bf16x8_t pf[NQ][TT];
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
@@ -199,28 +278,32 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
         p[k] = sx[(i * 4 + k) * 64 + lane];
 #pragma unroll
         for (int q = 1; q < KS; ++q) p[k] += sx[(i * 4 + q * KT + k) * 64 + lane];
-        p[k] *= a.scale_log2;
       }
+      seen[i] = 0xffffffffu;
       if (hide) {
+        seen[i] = 0;
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
           const int j = j0 + k * 16 + g * 4;
-          bool there = true;                                   // (4 keys, one page)
-          if (gap && j < k1) { const int e = tab[j >> a.shift]; there = e >= 0 && e < a.npages; }
+          const bool there = page_there(a, w, j);              // (4 keys, one page)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[k][e] = there && j + e <= pos[i] && j + e < k1 ? p[k][e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) {
+            const bool see = there && j + e <= pos[i] && j + e < w.k1;
+            p[k][e] = see ? p[k][e] : -INFINITY;
+            seen[i] |= (uint32_t)see << (k * 4 + e);
+          }
         }
       }
 #pragma unroll
       for (int k = 0; k < KT; ++k) mx = fmaxf(mx, fmaxf(fmaxf(p[k][0], p[k][1]), fmaxf(p[k][2], p[k][3])));
-      mx = gmax(mx);
+      mx = gmax(mx) * a.scale_log2;
       const float mn = fmaxf(m[i], mx), ms = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m[i] - ms);
       m[i] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { p[k][e] = __builtin_amdgcn_exp2f(p[k][e] - ms); sum += p[k][e]; }
+        for (int e = 0; e < 4; ++e) { p[k][e] = __builtin_amdgcn_exp2f(fmaf(p[k][e], a.scale_log2, -ms)); sum += p[k][e]; }
       l[i] = l[i] * f + sum;
       if (__any(f != 1.f)) {
 #pragma unroll
@@ -228,14 +311,14 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        u32x4_t w = {pack2bf(p[2 * t][0], p[2 * t][1]), pack2bf(p[2 * t][2], p[2 * t][3]), 0u, 0u};
-        if constexpr (KT > 1) { w[2] = pack2bf(p[2 * t + 1][0], p[2 * t + 1][1]); w[3] = pack2bf(p[2 * t + 1][2], p[2 * t + 1][3]); }
-        pf[i][t] = __builtin_bit_cast(bf16x8_t, w);
+        u32x4_t v = {pack2bf(p[2 * t][0], p[2 * t][1]), pack2bf(p[2 * t][2], p[2 * t][3]), 0u, 0u};
+        if constexpr (KT > 1) { v[2] = pack2bf(p[2 * t + 1][0], p[2 * t + 1][1]); v[3] = pack2bf(p[2 * t + 1][2], p[2 * t + 1][3]); }
+        pf[i][t] = __builtin_bit_cast(bf16x8_t, v);
       }
     }
     const uint32_t va = vaddr0 + stage * 2 * TILEB;
     auto product = [&](auto checked) {
-      constexpr int G = DT < 4 ? DT : 4;                         // fragments read ahead of their products
+      constexpr int G = DT < 4 ? DT : 4;                       // fragments read ahead of their products
 #pragma unroll
       for (int d0 = 0; d0 < DT; d0 += G) {
         bf16x8_t vf[G][TT];
@@ -253,57 +336,34 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
           for (int t = 0; t < TT; ++t) {
             asm volatile("" : "+v"(vf[d][t]));
             if constexpr (decltype(checked)::value) {
-              u32x4_t w = __builtin_bit_cast(u32x4_t, vf[d][t]);
+              if (__any(not_finite(vf[d][t]))) {
+                bf16x8_t code;
+                take_out(vf[d][t], code);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
-                if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu;
+                for (int i = 0; i < NQ; ++i) {
+                  const f32x4_t c = mfma16(code, seen8(KT > 1 ? seen[i] >> (8 * t) : seen[i] & 0xfu), (f32x4_t){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[i][d0 + d][e] = put_back(o[i][d0 + d][e], c[e]);
+                }
               }
-              vf[d][t] = __builtin_bit_cast(bf16x8_t, w);
             }
 #pragma unroll
             for (int i = 0; i < NQ; ++i) o[i][d0 + d] = mfma16(vf[d][t], pf[i][t], o[i][d0 + d]);
           }
       }
     };
-    if (!slow) product(std::false_type{});
-    else product(std::true_type{});
-    if (slow) {                                                // the values that are not finite, for the rows that see them
-      for (int k = 0; k < BN; ++k) {
-        const int j = j0 + k;
-        if (j >= k1) break;
-        bool there = true;
-        if (gap) { const int e = tab[j >> a.shift]; there = e >= 0 && e < a.npages; }
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          const int from = (k & 12) * 4 + c16;                 // the lane that holds this key's scores of this lane's row
-          float s = sx[(i * 4 + k / 16) * 64 + from][k & 3];
-#pragma unroll
-          for (int q = 1; q < KS; ++q) s += sx[(i * 4 + q * KT + k / 16) * 64 + from][k & 3];
-          const float p = fmaxf(__builtin_amdgcn_exp2f(s * a.scale_log2 - (m[i] == -INFINITY ? 0.f : m[i])), 1e-30f);
-          const bool see = there && j <= pos[i];
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const int col = wave * (HD / 4) + d * 16 + g * 4;
-            const u32x2_t w = *(const u32x2_t*)(kt + TILEB + k * ROWB + (((col >> 3) ^ tile_swz<HD>(k)) << 4) + (col & 7) * 2);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = e & 1 ? bfhi(w[e >> 1]) : bflo(w[e >> 1]);
-              if (see && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[i][d][e] += p * v;
-            }
-          }
-        }
-      }
-    }
+    // (a tile of which one row sees a key that another one does not: a value that is not finite must not reach the latter through its probability of 0)
+    if (first < last && j0 + BN - 1 > first) product(std::true_type{});
+    else product(std::false_type{});
   }
 
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
     const float lt = gsum(l[i]);
-    const int row = row0 + i * 16 + c16, tok = row / a.grp;
-    if (row >= rows) continue;
-    const int h = hk * a.grp + row - tok * a.grp;
-    const size_t t = t0 + tok;
+    const int row = w.row0 + i * 16 + c16, tok = row / a.grp;
+    if (row >= w.rows) continue;
+    const int h = w.hk * a.grp + row - tok * a.grp;
+    const size_t t = w.t0 + tok;
     if (a.nsplit == 1) {
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
@@ -312,7 +372,7 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
         if (col < a.hd) *(u32x2_t*)(a.out + t * a.ldo + (size_t)h * a.hd + col) = (u32x2_t){pack2bf(o[i][d][0] * inv, o[i][d][1] * inv), pack2bf(o[i][d][2] * inv, o[i][d][3] * inv)};
       }
     } else {
-      const size_t rid = ((size_t)sp * a.T + t) * a.H + h;
+      const size_t rid = ((size_t)w.sp * a.T + t) * a.H + h;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const int col = wave * (HD / 4) + d * 16 + g * 4;
@@ -321,6 +381,157 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
       if (wave == 0 && g == 0) { a.part_ml[rid * 2] = m[i]; a.part_ml[rid * 2 + 1] = lt; }
     }
   }
+}
+
+// ---- many rows: one workgroup (4 waves, 128 rows) per (kv head, tile of rows, split of the keys), heads of up to 128 columns -----------------------------------
+// Every wave has 32 rows of its own and goes through all keys of a tile with 32 x 32 x 16 products: S^T = K Q^T (a lane has one row and 16 of every 32 keys, so a
+// row's maximum and sum are 31 operations and one exchange of the wave's halves), P^T is already the right operand of O^T = V^T P^T.  No wave waits for another but
+// for the tile.  The running maximum follows only when a score passes it by more than 2^8: the probabilities then stay below 2^8, where bf16 and the fp32
+// sums are as exact as below 1, and the accumulators are rarely rescaled.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
+  constexpr int BN = 64, BM = 128, ROWB = HD * 2, TILEB = BN * ROWB, DS = HD / 16, DT = HD / 32;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
+  Work w;
+  if (!find_work(a, BM, lane, w)) return;
+  const int wrow = w.row0 + wave * 32, row = wrow + c32, tok = row / a.grp;
+  const bool mine = wrow < w.rows, ok = row < w.rows;
+  const int pos = ok ? w.kv - w.n + tok : -1;
+  const int first = row_pos(w, wrow, a.grp), last = mine ? row_pos(w, min(wrow + 32, w.rows) - 1, a.grp) : -1;      // of this wave's rows
+  bf16x8_t qf[DS];
+  {
+    const bf16_t* p = a.q + (size_t)(w.t0 + (ok ? tok : 0)) * a.ldq + (size_t)(w.hk * a.grp + (ok ? row - tok * a.grp : 0)) * a.hd;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      const int d = s * 16 + half * 8;
+      u32x4_t v = {0u, 0u, 0u, 0u};
+      if (ok && d < a.hd) v = read_q(a, p + d);
+      qf[s] = __builtin_bit_cast(bf16x8_t, v);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < DS; ++s) asm volatile("" : "+v"(qf[s]));
+  f32x16_t o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+  float m = -INFINITY, l = 0.f;                                // m: in units of the scaled scores, what the probabilities are relative to
+  const int krow = c32 * ROWB, kswz = swz32<HD>(c32);
+  const int vr = 4 * half + ((lane & 15) >> 2);                // row and columns of a lane in a transposing read: 4 rows x 16 columns per 16 lanes
+  const int vc = (lane & 16) + (lane & 3) * 4;
+  const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((vc >> 3) ^ swz32<HD>(vr)) << 4) + (vc & 7) * 2;
+
+  Copier<HD, BN, swz32<HD>> cp;
+  cp.init(a, wave, lane);
+  if (w.k0 < w.k1) { cp.pages(a, w, w.k0, wave); cp.issue(a, w, w.k0, smem, wave, lane); cp.pages(a, w, w.k0 + BN, wave); }
+  int stage = 0;
+  for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one
+    if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
+    if (j0 > last) continue;                                   // none of this wave's rows sees the tile
+    const char* kt = smem + stage * 2 * TILEB;
+    f32x16_t s[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[k][e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < DS; ++q) {
+        const bf16x8_t kf = *(const bf16x8_t*)(kt + k * 32 * ROWB + krow + (((2 * q + half) ^ kswz) << 4));
+        s[k] = mfma32(kf, qf[q], s[k]);
+      }
+    }
+    uint32_t seen = 0xffffffffu;                               // bit 16 k + e: key 32 k + 8 (e / 4) + 4 half + e % 4
+    if (w.gap || j0 + BN - 1 > first) {
+      seen = 0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int j = j0 + k * 32 + e4 * 8 + half * 4;
+          const bool there = page_there(a, w, j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool see = there && j + e <= pos && j + e < w.k1;
+            s[k][e4 * 4 + e] = see ? s[k][e4 * 4 + e] : -INFINITY;
+            seen |= (uint32_t)see << (k * 16 + e4 * 4 + e);
+          }
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2;
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m - ms);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    bf16x8_t pf[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) { s[k][e] = __builtin_amdgcn_exp2f(fmaf(s[k][e], a.scale_log2, -ms)); l += s[k][e]; }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        pf[2 * k + t] = __builtin_bit_cast(bf16x8_t, (u32x4_t){pack2bf(s[k][8 * t], s[k][8 * t + 1]), pack2bf(s[k][8 * t + 2], s[k][8 * t + 3]),
+                                                               pack2bf(s[k][8 * t + 4], s[k][8 * t + 5]), pack2bf(s[k][8 * t + 6], s[k][8 * t + 7])});
+    }
+    const uint32_t va = vaddr0 + stage * 2 * TILEB, vb = va ^ 32;       // rows + 8: the swizzle differs by two pieces
+    // (a tile of which one row sees a key that another one does not: a value that is not finite must not reach the latter through its probability of 0)
+    const bool uneven = first < last && j0 + BN - 1 > first;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      bf16x8_t vf[4];
+      const uint32_t x = va ^ (d * 64), y = vb ^ (d * 64);
+      vf[0] = tr_join(ds_read_tr_na<0>(x), ds_read_tr_na<8 * ROWB>(y));
+      vf[1] = tr_join(ds_read_tr_na<16 * ROWB>(x), ds_read_tr_na<24 * ROWB>(y));
+      vf[2] = tr_join(ds_read_tr_na<32 * ROWB>(x), ds_read_tr_na<40 * ROWB>(y));
+      vf[3] = tr_join(ds_read_tr_na<48 * ROWB>(x), ds_read_tr_na<56 * ROWB>(y));
+      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vf[0]), "+v"(vf[1]), "+v"(vf[2]), "+v"(vf[3])::"memory");
+      if (uneven) {
+        if (__any(not_finite(vf[0]) || not_finite(vf[1]) || not_finite(vf[2]) || not_finite(vf[3]))) {
+          f32x16_t c;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) c[e] = 0.f;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            bf16x8_t code;
+            take_out(vf[t], code);
+            c = mfma32(code, seen8(seen >> (8 * t)), c);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] = put_back(o[d][e], c[e]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[d] = mfma32(vf[t], pf[t], o[d]);
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!ok) return;
+  const int h = w.hk * a.grp + row - tok * a.grp;
+  const size_t t = w.t0 + tok;
+  const size_t rid = ((size_t)w.sp * a.T + t) * a.H + h;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int col = d * 32 + e * 8 + half * 4;
+      if (col >= a.hd) continue;
+      const f32x4_t v = {o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+      if (a.nsplit == 1) *(u32x2_t*)(a.out + t * a.ldo + (size_t)h * a.hd + col) = (u32x2_t){pack2bf(v[0] * inv, v[1] * inv), pack2bf(v[2] * inv, v[3] * inv)};
+      else *(f32x4_t*)(a.part_o + rid * a.hd + col) = v;
+    }
+  if (a.nsplit > 1 && half == 0) { a.part_ml[rid * 2] = m; a.part_ml[rid * 2 + 1] = l; }
 }
 
 // The partial results of the splits that a row's keys reach, joined in their order: weights 2^(m_z - max m), fp32.
@@ -352,16 +563,15 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
 }
 
 // ---- choices on the host, from sizes alone -----------------------------------------------------------------------------------------------------------
-struct Choice { int hd, nq, bn, nsplit, cmin; long tiles; };
+struct Choice { int hd, nq, nsplit, cmin; long tiles; };
 
 Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, int cu_count) {
   Choice c;
   c.hd = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : hd <= 512 ? 512 : 1024;
   const int grp = H / Hkv;
   const long rows = (max_new > 0 && max_new < T ? max_new : (T + R - 1) / R) * grp;      // rows of a stream and kv head
-  c.nq = rows <= 16 || c.hd == 1024 ? 1 : c.hd == 512 ? 2 : 4;
-  c.bn = c.hd <= 128 ? 64 : c.hd <= 512 ? 32 : 16;
-  c.tiles = (long)T * grp / (16 * c.nq) + R;
+  c.nq = rows <= 16 || c.hd == 1024 ? 1 : c.hd == 512 ? 2 : c.hd == 256 ? 4 : 0;      // 0: the kernel for many rows
+  c.tiles = (long)T * grp / (c.nq ? 16 * c.nq : 128) + R;
   c.cmin = 256;
   const long items = c.tiles * Hkv;
   long want = (2l * cu_count + items - 1) / items, most = (max_kv + c.cmin - 1) / c.cmin;
@@ -375,13 +585,18 @@ long part_floats(const Choice& c, long T, long H, long hd) { return c.nsplit > 1
 
 template <int HD, int NQ, int BN>
 int launch_tiles(const AttnArgs& a, const Choice& c, hipStream_t st) {
-  constexpr int lds = 4 * BN * HD * 2 + NQ * 4096 + 64;
+  constexpr int lds = 4 * BN * HD * 2 + NQ * 4096;
   static_assert(lds <= 160 * 1024, "LDS");
   if constexpr (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_tile_kernel<HD, NQ, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     AVT_CHECK(e == hipSuccess, "avt_paged_attn_fwd: %s", hipGetErrorString(e));
   }
   hipLaunchKernelGGL((paged_attn_tile_kernel<HD, NQ, BN>), dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(256), lds, st, a);
+  return 0;
+}
+template <int HD>
+int launch_long(const AttnArgs& a, const Choice& c, hipStream_t st) {
+  hipLaunchKernelGGL((paged_attn_long_kernel<HD>), dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(256), 4 * 64 * HD * 2, st, a);
   return 0;
 }
 constexpr int CUS = 256;
@@ -412,12 +627,13 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   a.q = (const bf16_t*)q; a.kc = (const bf16_t*)kcache; a.vc = (const bf16_t*)vcache; a.table = table; a.cu = cu; a.kv_lens = kv_lens; a.out = (bf16_t*)out;
   a.part_o = (float*)ws; a.part_ml = (float*)ws + (size_t)c.nsplit * T * H * head_dim;
   a.ldq = ldq; a.ldo = ldo; a.npages = npages; a.shift = __builtin_ctz(page); a.ldt = ldt; a.width = width; a.T = T; a.R = R; a.H = H; a.Hkv = Hkv; a.grp = H / Hkv;
-  a.hd = head_dim; a.nsplit = c.nsplit; a.cmin = c.cmin; a.scale_log2 = scale * 1.4426950408889634f;
+  a.hd = head_dim; a.nsplit = c.nsplit; a.cmin = c.cmin; a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
+  a.q_and = scale == 0.f ? 0u : 0xffffffffu; a.q_xor = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t st = (hipStream_t)stream;
   int rc = 0;
   if (c.nq == 1) rc = c.hd == 64 ? launch_tiles<64, 1, 64>(a, c, st) : c.hd == 128 ? launch_tiles<128, 1, 64>(a, c, st) : c.hd == 256 ? launch_tiles<256, 1, 32>(a, c, st)
                     : c.hd == 512 ? launch_tiles<512, 1, 32>(a, c, st) : launch_tiles<1024, 1, 16>(a, c, st);
-  else rc = c.hd == 64 ? launch_tiles<64, 4, 64>(a, c, st) : c.hd == 128 ? launch_tiles<128, 4, 64>(a, c, st) : c.hd == 256 ? launch_tiles<256, 4, 32>(a, c, st)
+  else rc = c.hd == 64 ? launch_long<64>(a, c, st) : c.hd == 128 ? launch_long<128>(a, c, st) : c.hd == 256 ? launch_tiles<256, 4, 32>(a, c, st)
           : launch_tiles<512, 2, 32>(a, c, st);
   if (rc) return rc;
   AVT_LAUNCH_CHECK();

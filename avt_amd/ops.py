@@ -714,15 +714,15 @@ def _refuse(msg):
 
 def _here(first, *tensors):
     """Every tensor on the current device: the kernels go to its current stream, which is returned."""
-    dev = first.device
+    dev = first.get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            _refuse(f'tensors on different devices ({dev}, {t.device})')
-    if dev.type != 'cuda':
-        _refuse(f'tensors must live on a GPU, got {dev} (no CPU fallback exists)')
-    if dev.index != torch.cuda.current_device():
-        _refuse(f'tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}')
-    return torch._C._cuda_getCurrentRawStream(dev.index)       # (the handle alone: torch.cuda.current_stream() builds an object around it, 2 us of a call of 10)
+        if t is not None and t.get_device() != dev:
+            _refuse(f'tensors on different devices ({first.device}, {t.device})')
+    if dev < 0 or not first.is_cuda:
+        _refuse(f'tensors must live on a GPU, got {first.device} (no CPU fallback exists)')
+    if dev != torch.cuda.current_device():
+        _refuse(f'tensors on cuda:{dev}, but the current device is cuda:{torch.cuda.current_device()}')
+    return torch._C._cuda_getCurrentRawStream(dev)             # (the handle alone: torch.cuda.current_stream() builds an object around it, 2 us of a call of 10)
 
 
 def _ints(n, name, t):
