@@ -1,12 +1,12 @@
 // Causal attention of each stream's new tokens over its pages of a shared key / value cache (HF GPT-2 attention with past_key_values, for streams of
 // different lengths): query i of a stream with n new tokens and kv cached ones (the new ones among them) sits at position x = kv - n + i and sees the
 // keys 0 .. x:  o = sum_{j <= x} softmax_j(scale q k_j) v_j, and 0 where x < 0.
-#include <type_traits>
+#include <algorithm>
 #include "common.hpp"
 #include "../../include/avt_hip.h"
 
 namespace {
-constexpr int HDMAX = 1024;
+constexpr int HDMAX = 1024, MAX_SPLITS = 128, FEW_SPLITS = 4;
 
 // The stream whose new tokens hold row t: the last r with cu[r] <= t, and t < cu[r + 1]; -1 behind the last stream.  All 64 lanes probe at once.
 __device__ __forceinline__ int find_stream(const int* __restrict__ cu, int R, int t, int lane) {
@@ -61,91 +61,98 @@ __device__ __forceinline__ float gmax(float v) { v = fmaxf(v, __shfl_xor(v, 16, 
 // Tile i of a stream's rows (a row = a new token and one of the query heads that share the kv head) is tile cu[r] * grp / BM + r + i of the grid: the tiles of
 // two streams never meet, the sum over the streams is known on the host from T and R, and no list of tiles has to be made.
 __device__ __forceinline__ int tile_base(const int* __restrict__ cu, int r, int T, int grp, int bm) { return max(0, min(cu[r], T)) * grp / bm + r; }
-__device__ __forceinline__ int find_tile(const int* __restrict__ cu, int R, int T, int grp, int bm, int tile, int lane) {
-  int lo = 0, hi = R;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64;
-    const int p = lo + lane * step;
-    const int c = __popcll(__ballot(p < hi && tile_base(cu, p < hi ? p : lo, T, grp, bm) <= tile));
-    lo += (c > 0 ? c - 1 : 0) * step;
-    hi = min(lo + step, hi);
-  }
-  return lo;
-}
-
-__device__ __forceinline__ u32x4_t read_q(const AttnArgs& a, const bf16_t* p) {
-  u32x4_t v = *(const u32x4_t*)p;
+// q as it was read -> the operand: zeros where there is no row or no column
+__device__ __forceinline__ void prepare_q(const AttnArgs& a, bf16x8_t& q, bool there) {
+  u32x4_t v = __builtin_bit_cast(u32x4_t, q);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (v[e] & a.q_and) ^ a.q_xor;
-  return v;
+  for (int e = 0; e < 4; ++e) v[e] = there ? (v[e] & a.q_and) ^ a.q_xor : 0u;
+  q = __builtin_bit_cast(bf16x8_t, v);
+  asm volatile("" : "+v"(q));
 }
 
 // What a workgroup works on: rows row0 .. of a stream's `rows`, keys k0 .. k1 - 1.
 struct Work {
   int hk, sp, t0, n, row0, rows, kv, k0, k1;
   bool gap;                                                    // some table entry of the range names no page
+  int entry;                                                   // this lane's entry of the range (its first 64)
   table_t tab;
 };
 __device__ __forceinline__ int row_pos(const Work& w, int row, int grp) { return w.kv - w.n + row / grp; }
+// (All 64 lanes probe at once, and the last probe brings the stream's numbers with it: what a workgroup waits for before its first copy is this, the page and no more.)
 __device__ __forceinline__ bool find_work(const AttnArgs& a, int bm, int lane, Work& w) {
   w.hk = blockIdx.x % a.Hkv;
   w.sp = blockIdx.y;
   const int tile = (gridDim.x - 1 - blockIdx.x) / a.Hkv;       // (the last rows of a chunk see the most keys: first)
-  const int r = __builtin_amdgcn_readfirstlane(find_tile(a.cu, a.R, a.T, a.grp, bm, tile, lane));
-  w.t0 = max(0, min(a.cu[r], a.T));
-  w.n = max(0, min(a.cu[r + 1], a.T) - w.t0);
-  w.row0 = (tile - tile_base(a.cu, r, a.T, a.grp, bm)) * bm;
+  int lo = 0, hi = a.R;
+  while (hi - lo > 64) {
+    const int step = (hi - lo + 63) / 64;
+    const int p = lo + lane * step;
+    const int c = __popcll(__ballot(p < hi && tile_base(a.cu, p < hi ? p : lo, a.T, a.grp, bm) <= tile));
+    lo += (c > 0 ? c - 1 : 0) * step;
+    hi = min(lo + step, hi);
+  }
+  const int p = min(lo + lane, a.R - 1);
+  const int c0 = max(0, min(a.cu[p], a.T)), c1 = max(0, min(a.cu[p + 1], a.T)), len = a.kv_lens[p];
+  const int base = c0 * a.grp / bm + p;
+  const int hit = max(__popcll(__ballot(lo + lane < hi && base <= tile)) - 1, 0);
+  const int r = __builtin_amdgcn_readfirstlane(lo + hit);
+  w.t0 = __builtin_amdgcn_readlane(c0, hit);
+  w.n = max(0, __builtin_amdgcn_readlane(c1, hit) - w.t0);
+  w.row0 = (tile - __builtin_amdgcn_readlane(base, hit)) * bm;
   w.rows = w.n * a.grp;
   if (w.row0 < 0 || w.row0 >= w.rows) return false;
-  w.kv = (int)min((long)max(a.kv_lens[r], 0), (long)a.width << a.shift);
+  w.kv = (int)min((long)max(__builtin_amdgcn_readlane(len, hit), 0), (long)a.width << a.shift);
   const int last = row_pos(w, min(w.row0 + bm, w.rows) - 1, a.grp);
   const long chunk = split_keys(w.kv, a.nsplit, a.cmin);
   w.k0 = (int)min((long)w.sp * chunk, (long)w.kv);
   w.k1 = (int)min((long)(w.sp + 1) * chunk, (long)(last + 1));
   if (w.k0 >= w.k1 && a.nsplit > 1) return false;              // (the join knows)
   w.tab = (table_t)(a.table + (size_t)r * a.ldt);
-  bool gap = false;
-  if (w.k0 < w.k1)
-    for (int e = (w.k0 >> a.shift) + lane; e <= (w.k1 - 1) >> a.shift; e += 64) { const int pg = a.table[(size_t)r * a.ldt + e]; gap |= pg < 0 || pg >= a.npages; }
-  w.gap = __any(gap);
+  w.gap = true;                                                // until find_gap, which nothing waits for before the first copies are out
+  w.entry = w.tab[max(0, min((w.k0 >> a.shift) + lane, (w.k1 - 1) >> a.shift))];
   return true;
 }
+__device__ __forceinline__ void find_gap(const AttnArgs& a, int lane, Work& w) {
+  bool gap = w.entry < 0 || w.entry >= a.npages;
+  for (int e = (w.k0 >> a.shift) + 64 + lane; e <= (w.k1 - 1) >> a.shift; e += 64) { const int pg = w.tab[e]; gap |= pg < 0 || pg >= a.npages; }
+  w.gap = __any(gap);
+}
 
-// Copies of K and V tiles of BN keys into LDS by 4 waves, 1 KB an instruction: its rows lie in one page (a page holds at least 8 tokens), so the page's address is
-// scalar and a lane's offset within it does not change from tile to tile.  Rows behind the last key, rows of no page and columns behind the head's are asked for
-// out of range and arrive as zeros: what is not finite in memory that holds no key never meets a probability of 0.
+// Copies of K and V tiles of BN keys into LDS by 4 waves, 1 KB an instruction.  A wave copies a quarter of the tile's rows, which lie in one page (two, where they
+// are 16 and a page may hold 8): the pages' addresses are scalar, and what a lane adds to them does not change from tile to tile, so a copy is little more than its own
+// instruction.  Rows behind the last key, rows of no page and columns behind the head's are asked for out of range and arrive as zeros: what is not
+// finite in memory that holds no key never meets a probability of 0.
 template <int HD, int BN, int (*SWZ)(int)>
 struct Copier {
-  static constexpr int ROWB = HD * 2, TILEB = BN * ROWB, NI = TILEB / 4096;
+  static constexpr int ROWB = HD * 2, TILEB = BN * ROWB, NI = TILEB / 4096, RW = BN / 4, PG = RW > 8 ? 2 : 1, RP = RW / PG;      // rows of a wave, of a page's part
   static constexpr uint32_t NONE = 0xFFFFFFF0u;
-  uint32_t off[NI];
-  int pg[NI];
+  uint32_t off[NI];                                            // of the lane's 16 bytes from its part's first row
+  int pg[PG];
   __device__ __forceinline__ void init(const AttnArgs& a, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int at = (i * 4 + wave) * 1024 + lane * 16, row = at / ROWB, c = ((at % ROWB) >> 4) ^ SWZ(row);
-      off[i] = c * 8 < a.hd ? (uint32_t)(((row - (i * 4 + wave) * 1024 / ROWB) * a.Hkv * a.hd + c * 8) * 2) : NONE;
+      const int at = i * 1024 + lane * 16, row = at / ROWB, c = ((at % ROWB) >> 4) ^ SWZ(wave * RW + row);
+      off[i] = c * 8 < a.hd ? (uint32_t)(((row % RP) * a.Hkv * a.hd + c * 8) * 2) : NONE;
     }
   }
   __device__ __forceinline__ void pages(const AttnArgs& a, const Work& w, int j0, int wave) {      // of the tile that is issued next
-    if (j0 < w.k1) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) pg[i] = w.tab[min(j0 + (i * 4 + wave) * 1024 / ROWB, w.k1 - 1) >> a.shift];
-    }
+    for (int q = 0; q < PG; ++q) pg[q] = w.tab[max(0, min(j0 + wave * RW + q * RP, w.k1 - 1)) >> a.shift];
   }
   __device__ __forceinline__ void issue(const AttnArgs& a, const Work& w, int j0, char* dst, int wave, int lane) {
     const bool whole = j0 + BN <= w.k1 && !w.gap;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int jb = j0 + (i * 4 + wave) * 1024 / ROWB;
-      uint32_t v = off[i];
-      if (!whole) {
-        const int row = ((i * 4 + wave) * 1024 + lane * 16) / ROWB;
-        if (j0 + row >= w.k1 || pg[i] < 0 || pg[i] >= a.npages) v = NONE;
+    for (int q = 0; q < PG; ++q) {
+      const int jb = j0 + wave * RW + q * RP;
+      const size_t at = ((((size_t)(uint32_t)pg[q] << a.shift) + (jb & ((1 << a.shift) - 1))) * a.Hkv + w.hk) * a.hd;
+      const bool there = pg[q] >= 0 && pg[q] < a.npages;
+#pragma unroll
+      for (int i = q * NI / PG; i < (q + 1) * NI / PG; ++i) {
+        uint32_t v = off[i];
+        if (!whole && (jb + (i * 1024 + lane * 16) / ROWB % RP >= w.k1 || !there)) v = NONE;
+        copy(a.kc + at, dst + wave * (TILEB / 4) + i * 1024, v);
+        copy(a.vc + at, dst + TILEB + wave * (TILEB / 4) + i * 1024, v);
       }
-      const size_t at = ((((size_t)(uint32_t)pg[i] << a.shift) + (jb & ((1 << a.shift) - 1))) * a.Hkv + w.hk) * a.hd;
-      copy(a.kc + at, dst + (i * 4 + wave) * 1024, v);
-      copy(a.vc + at, dst + TILEB + (i * 4 + wave) * 1024, v);
     }
   }
   __device__ __forceinline__ static void copy(const bf16_t* base, char* lds, uint32_t voff) {
@@ -190,197 +197,157 @@ __device__ __forceinline__ bf16x8_t seen8(uint32_t bits) {     // 8 bits -> 1.0 
   for (int e = 0; e < 4; ++e) w[e] = ((bits >> (2 * e)) & 1u ? 0x3f80u : 0u) | ((bits >> (2 * e + 1)) & 1u ? 0x3f800000u : 0u);
   return __builtin_bit_cast(bf16x8_t, w);
 }
+// Four columns of a row: the result, or this split's part of it
+__device__ __forceinline__ void put_out(const AttnArgs& a, size_t t, int h, size_t rid, int col, f32x4_t v, float inv) {
+  if (col >= a.hd) return;
+  if (a.nsplit == 1) *(u32x2_t*)(a.out + t * a.ldo + (size_t)h * a.hd + col) = (u32x2_t){pack2bf(v[0] * inv, v[1] * inv), pack2bf(v[2] * inv, v[3] * inv)};
+  else *(f32x4_t*)(a.part_o + rid * a.hd + col) = v;
+}
 __device__ __forceinline__ bool page_there(const AttnArgs& a, const Work& w, int j) {
   if (!w.gap || j >= w.k1) return true;
   const int e = w.tab[j >> a.shift];
   return e >= 0 && e < a.npages;
 }
 
-// ---- few rows: one workgroup (4 waves) per (kv head, tile of NQ * 16 rows, split of the keys) ------------------------------------------------------------------
+// ---- few rows: one workgroup (4 waves) per (kv head, tile of 16 rows, split of the keys) ------------------------------------------------------------------------
 // K and V tiles of BN keys, two in turn.  S^T = K Q^T: wave w takes 16 keys (w % KT) of the tile and, where the tile has fewer than 64 keys, its share of the head's
 // columns (w / KT); the scores pass through LDS (16 bytes per lane, the same lane reads them) and every wave then has all of them in the layout of P^T, the right
 // operand of O^T = V^T P^T, and keeps the running maximum and sum (fp32) of every row for itself: no reduction between waves.  Wave w owns a quarter of the head's
 // columns of O.  P is rounded to bf16 for the product (the matrix unit's type; half a step 2^-8 of each probability), the sum is of the unrounded ones.
-template <int HD, int NQ, int BN>
+template <int HD, int BN>
 __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
-  constexpr int ROWB = HD * 2, TILEB = BN * ROWB, KT = BN / 16, KS = 4 / KT, DS = HD / KS / 32, DT = HD / 64, TT = BN >= 32 ? BN / 32 : 1, BM = NQ * 16;
+  constexpr int ROWB = HD * 2, TILEB = BN * ROWB, KT = BN / 16, KS = 4 / KT, DS = HD / KS / 32, DT = HD / 64, TT = BN >= 32 ? BN / 32 : 1, BM = 16;
   static_assert(KT * KS == 4 && DS >= 1 && TILEB >= 4096, "tile shape");
   extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V], scores
-  f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [NQ][4 waves][64 lanes]
+  f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [4 waves][64 lanes]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g = lane >> 4;
   Work w;
   if (!find_work(a, BM, lane, w)) return;
   const int first = row_pos(w, w.row0, a.grp), last = row_pos(w, min(w.row0 + BM, w.rows) - 1, a.grp);
-
-  int pos[NQ];                                                 // this lane's row (column of S^T): its position, -1: no row
-  bf16x8_t qf[NQ][DS];
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const int row = w.row0 + i * 16 + c16, tok = row / a.grp;
-    const bool ok = row < w.rows;
-    pos[i] = ok ? w.kv - w.n + tok : -1;
+  const int row = w.row0 + c16, tok = row / a.grp;             // this lane's row (column of S^T)
+  const bool ok = row < w.rows;
+  const int pos = ok ? w.kv - w.n + tok : -1;
+  bf16x8_t qf[DS];
+  {
     const bf16_t* p = a.q + (size_t)(w.t0 + (ok ? tok : 0)) * a.ldq + (size_t)(w.hk * a.grp + (ok ? row - tok * a.grp : 0)) * a.hd;
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       const int d = (wave / KT) * (HD / KS) + s * 32 + g * 8;
-      u32x4_t v = {0u, 0u, 0u, 0u};
-      if (ok && d < a.hd) v = read_q(a, p + d);
-      qf[i][s] = __builtin_bit_cast(bf16x8_t, v);
+      qf[s] = *(const bf16x8_t*)(p + (d < a.hd ? d : 0));
     }
   }
-  f32x4_t o[NQ][DT];
-  float m[NQ], l[NQ];
+  f32x4_t o[DT];
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    m[i] = -INFINITY; l[i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[i][d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < DT; ++d) o[d] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   const int kswz = swz16<HD>(c16);
   const int krow = ((wave % KT) * 16 + c16) * ROWB, kc0 = (wave / KT) * (HD / KS / 8) + g;
   const int vr = 4 * g + (c16 >> 2);
   const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((wave * (HD / 32) + ((c16 & 3) >> 1)) ^ swz16<HD>(vr)) << 4) + (c16 & 1) * 8;
 
-  // (Q is waited for here: left to the first product, the compiler's wait for it would sit inside the loop and wait for the copies in flight as well)
-#pragma unroll
-  for (int i = 0; i < NQ; ++i)
-#pragma unroll
-    for (int s = 0; s < DS; ++s) asm volatile("" : "+v"(qf[i][s]));
   Copier<HD, BN, swz16<HD>> cp;
   cp.init(a, wave, lane);
-  if (w.k0 < w.k1) { cp.pages(a, w, w.k0, wave); cp.issue(a, w, w.k0, smem, wave, lane); cp.pages(a, w, w.k0 + BN, wave); }
+  cp.pages(a, w, w.k0, wave);
+  if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
+  cp.pages(a, w, w.k0 + BN, wave);
+  // (Q is waited for here: left to the first product, the compiler's wait for it would sit inside the loop and wait for the copies in flight as well)
+#pragma unroll
+  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], ok && (wave / KT) * (HD / KS) + s * 32 + g * 8 < a.hd);
+  find_gap(a, lane, w);
   int stage = 0;
   for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one and with the scores
     if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
     const char* kt = smem + stage * 2 * TILEB;
-    f32x4_t s4[NQ];
+    f32x4_t s4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) s4[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      const bf16x8_t kf = *(const bf16x8_t*)(kt + krow + (((kc0 + 4 * s) ^ kswz) << 4));
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) s4[i] = mfma16(kf, qf[i][s], s4[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) sx[(i * 4 + wave) * 64 + lane] = s4[i];
+    for (int s = 0; s < DS; ++s) s4 = mfma16(*(const bf16x8_t*)(kt + krow + (((kc0 + 4 * s) ^ kswz) << 4)), qf[s], s4);
+    sx[wave * 64 + lane] = s4;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const bool hide = w.gap || j0 + BN - 1 > first;            // some row does not see some key of this tile
-    uint32_t seen[NQ];
-    bf16x8_t pf[NQ][TT];
+    f32x4_t p[KT];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      f32x4_t p[KT];
-      float mx = -INFINITY;
+    for (int k = 0; k < KT; ++k) {
+      p[k] = sx[k * 64 + lane];
+#pragma unroll
+      for (int q = 1; q < KS; ++q) p[k] += sx[(q * KT + k) * 64 + lane];
+    }
+    uint32_t seen = 0xffffffffu;                               // bit 4 k + e: key 16 k + 4 g + e
+    if (w.gap || j0 + BN - 1 > first) {                        // some row does not see some key of this tile
+      seen = 0;
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
-        p[k] = sx[(i * 4 + k) * 64 + lane];
+        const int j = j0 + k * 16 + g * 4;
+        const bool there = page_there(a, w, j);                // (4 keys, one page)
 #pragma unroll
-        for (int q = 1; q < KS; ++q) p[k] += sx[(i * 4 + q * KT + k) * 64 + lane];
-      }
-      seen[i] = 0xffffffffu;
-      if (hide) {
-        seen[i] = 0;
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          const int j = j0 + k * 16 + g * 4;
-          const bool there = page_there(a, w, j);              // (4 keys, one page)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool see = there && j + e <= pos[i] && j + e < w.k1;
-            p[k][e] = see ? p[k][e] : -INFINITY;
-            seen[i] |= (uint32_t)see << (k * 4 + e);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const bool see = there && j + e <= pos && j + e < w.k1;
+          p[k][e] = see ? p[k][e] : -INFINITY;
+          seen |= (uint32_t)see << (k * 4 + e);
         }
       }
+    }
+    float mx = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < KT; ++k) mx = fmaxf(mx, fmaxf(fmaxf(p[k][0], p[k][1]), fmaxf(p[k][2], p[k][3])));
-      mx = gmax(mx) * a.scale_log2;
-      const float mn = fmaxf(m[i], mx), ms = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m[i] - ms);
-      m[i] = mn;
-      float sum = 0.f;
+    for (int k = 0; k < KT; ++k) mx = fmaxf(mx, fmaxf(fmaxf(p[k][0], p[k][1]), fmaxf(p[k][2], p[k][3])));
+    mx = gmax(mx) * a.scale_log2;
+    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m - ms);
+    m = mn;
+    float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < KT; ++k)
+    for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { p[k][e] = __builtin_amdgcn_exp2f(fmaf(p[k][e], a.scale_log2, -ms)); sum += p[k][e]; }
-      l[i] = l[i] * f + sum;
-      if (__any(f != 1.f)) {
+      for (int e = 0; e < 4; ++e) { p[k][e] = __builtin_amdgcn_exp2f(fmaf(p[k][e], a.scale_log2, -ms)); sum += p[k][e]; }
+    l = l * f + sum;
+    if (__any(f != 1.f)) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[i][d] *= f;
-      }
+      for (int d = 0; d < DT; ++d) o[d] *= f;
+    }
+    bf16x8_t pf[TT];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        u32x4_t v = {pack2bf(p[2 * t][0], p[2 * t][1]), pack2bf(p[2 * t][2], p[2 * t][3]), 0u, 0u};
-        if constexpr (KT > 1) { v[2] = pack2bf(p[2 * t + 1][0], p[2 * t + 1][1]); v[3] = pack2bf(p[2 * t + 1][2], p[2 * t + 1][3]); }
-        pf[i][t] = __builtin_bit_cast(bf16x8_t, v);
-      }
+    for (int t = 0; t < TT; ++t) {
+      u32x4_t v = {pack2bf(p[2 * t][0], p[2 * t][1]), pack2bf(p[2 * t][2], p[2 * t][3]), 0u, 0u};
+      if constexpr (KT > 1) { v[2] = pack2bf(p[2 * t + 1][0], p[2 * t + 1][1]); v[3] = pack2bf(p[2 * t + 1][2], p[2 * t + 1][3]); }
+      pf[t] = __builtin_bit_cast(bf16x8_t, v);
     }
     const uint32_t va = vaddr0 + stage * 2 * TILEB;
-    auto product = [&](auto checked) {
-      constexpr int G = DT < 4 ? DT : 4;                       // fragments read ahead of their products
-#pragma unroll
-      for (int d0 = 0; d0 < DT; d0 += G) {
-        bf16x8_t vf[G][TT];
-#pragma unroll
-        for (int d = 0; d < G; ++d) {
-          const uint32_t ad = (va ^ (((d0 + d) & 7) * 32)) + ((d0 + d) >> 3) * 256;
-          if constexpr (BN == 16) vf[d][0] = tr_join(ds_read_tr_na<0>(ad), (u32x2_t){0u, 0u});
-          else vf[d][0] = tr_join(ds_read_tr_na<0>(ad), ds_read_tr_na<16 * ROWB>(ad));
-          if constexpr (TT > 1) vf[d][TT - 1] = tr_join(ds_read_tr_na<(BN > 32 ? 32 : 0) * ROWB>(ad), ds_read_tr_na<(BN > 32 ? 48 : 0) * ROWB>(ad));
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int d = 0; d < G; ++d)
-#pragma unroll
-          for (int t = 0; t < TT; ++t) {
-            asm volatile("" : "+v"(vf[d][t]));
-            if constexpr (decltype(checked)::value) {
-              if (__any(not_finite(vf[d][t]))) {
-                bf16x8_t code;
-                take_out(vf[d][t], code);
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                  const f32x4_t c = mfma16(code, seen8(KT > 1 ? seen[i] >> (8 * t) : seen[i] & 0xfu), (f32x4_t){0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) o[i][d0 + d][e] = put_back(o[i][d0 + d][e], c[e]);
-                }
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) o[i][d0 + d] = mfma16(vf[d][t], pf[i][t], o[i][d0 + d]);
-          }
-      }
-    };
     // (a tile of which one row sees a key that another one does not: a value that is not finite must not reach the latter through its probability of 0)
-    if (first < last && j0 + BN - 1 > first) product(std::true_type{});
-    else product(std::false_type{});
-  }
-
+    const bool uneven = first < last && j0 + BN - 1 > first;
+    constexpr int G = DT < 4 ? DT : 4;                         // fragments read ahead of their products
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    const float lt = gsum(l[i]);
-    const int row = w.row0 + i * 16 + c16, tok = row / a.grp;
-    if (row >= w.rows) continue;
-    const int h = w.hk * a.grp + row - tok * a.grp;
-    const size_t t = w.t0 + tok;
-    if (a.nsplit == 1) {
-      const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    for (int d0 = 0; d0 < DT; d0 += G) {
+      bf16x8_t vf[G][TT];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int col = wave * (HD / 4) + d * 16 + g * 4;
-        if (col < a.hd) *(u32x2_t*)(a.out + t * a.ldo + (size_t)h * a.hd + col) = (u32x2_t){pack2bf(o[i][d][0] * inv, o[i][d][1] * inv), pack2bf(o[i][d][2] * inv, o[i][d][3] * inv)};
+      for (int d = 0; d < G; ++d) {
+        const uint32_t ad = (va ^ (((d0 + d) & 7) * 32)) + ((d0 + d) >> 3) * 256;
+        if constexpr (BN == 16) vf[d][0] = tr_join(ds_read_tr_na<0>(ad), (u32x2_t){0u, 0u});
+        else vf[d][0] = tr_join(ds_read_tr_na<0>(ad), ds_read_tr_na<16 * ROWB>(ad));
+        if constexpr (TT > 1) vf[d][TT - 1] = tr_join(ds_read_tr_na<(BN > 32 ? 32 : 0) * ROWB>(ad), ds_read_tr_na<(BN > 32 ? 48 : 0) * ROWB>(ad));
       }
-    } else {
-      const size_t rid = ((size_t)w.sp * a.T + t) * a.H + h;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int col = wave * (HD / 4) + d * 16 + g * 4;
-        if (col < a.hd) *(f32x4_t*)(a.part_o + rid * a.hd + col) = o[i][d];
-      }
-      if (wave == 0 && g == 0) { a.part_ml[rid * 2] = m[i]; a.part_ml[rid * 2 + 1] = lt; }
+      for (int d = 0; d < G; ++d)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          asm volatile("" : "+v"(vf[d][t]));
+          if (uneven && __any(not_finite(vf[d][t]))) {
+            bf16x8_t code;
+            take_out(vf[d][t], code);
+            const f32x4_t c = mfma16(code, seen8(KT > 1 ? seen >> (8 * t) : seen & 0xfu), (f32x4_t){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[d0 + d][e] = put_back(o[d0 + d][e], c[e]);
+          }
+          o[d0 + d] = mfma16(vf[d][t], pf[t], o[d0 + d]);
+        }
     }
   }
+  l = gsum(l);
+  if (!ok) return;
+  const int h = w.hk * a.grp + row - tok * a.grp;
+  const size_t t = w.t0 + tok, rid = ((size_t)w.sp * a.T + t) * a.H + h;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) put_out(a, t, h, rid, wave * (HD / 4) + d * 16 + g * 4, o[d], inv);
+  if (a.nsplit > 1 && wave == 0 && g == 0) { a.part_ml[rid * 2] = m; a.part_ml[rid * 2 + 1] = l; }
 }
 
 // ---- many rows: one workgroup (4 waves, 128 rows) per (kv head, tile of rows, split of the keys), heads of up to 128 columns -----------------------------------
@@ -405,13 +372,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       const int d = s * 16 + half * 8;
-      u32x4_t v = {0u, 0u, 0u, 0u};
-      if (ok && d < a.hd) v = read_q(a, p + d);
-      qf[s] = __builtin_bit_cast(bf16x8_t, v);
+      qf[s] = *(const bf16x8_t*)(p + (d < a.hd ? d : 0));
     }
   }
-#pragma unroll
-  for (int s = 0; s < DS; ++s) asm volatile("" : "+v"(qf[s]));
   f32x16_t o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -425,7 +388,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
 
   Copier<HD, BN, swz32<HD>> cp;
   cp.init(a, wave, lane);
-  if (w.k0 < w.k1) { cp.pages(a, w, w.k0, wave); cp.issue(a, w, w.k0, smem, wave, lane); cp.pages(a, w, w.k0 + BN, wave); }
+  cp.pages(a, w, w.k0, wave);
+  if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
+  cp.pages(a, w, w.k0 + BN, wave);
+#pragma unroll
+  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], ok && s * 16 + half * 8 < a.hd);
+  find_gap(a, lane, w);
   int stage = 0;
   for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one
@@ -518,33 +486,179 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
   l += __shfl_xor(l, 32, 64);
   if (!ok) return;
   const int h = w.hk * a.grp + row - tok * a.grp;
-  const size_t t = w.t0 + tok;
-  const size_t rid = ((size_t)w.sp * a.T + t) * a.H + h;
+  const size_t t = w.t0 + tok, rid = ((size_t)w.sp * a.T + t) * a.H + h;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int col = d * 32 + e * 8 + half * 4;
-      if (col >= a.hd) continue;
-      const f32x4_t v = {o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
-      if (a.nsplit == 1) *(u32x2_t*)(a.out + t * a.ldo + (size_t)h * a.hd + col) = (u32x2_t){pack2bf(v[0] * inv, v[1] * inv), pack2bf(v[2] * inv, v[3] * inv)};
-      else *(f32x4_t*)(a.part_o + rid * a.hd + col) = v;
-    }
+    for (int e = 0; e < 4; ++e) put_out(a, t, h, rid, d * 32 + e * 8 + half * 4, (f32x4_t){o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]}, inv);
   if (a.nsplit > 1 && half == 0) { a.part_ml[rid * 2] = m; a.part_ml[rid * 2 + 1] = l; }
 }
 
-// The partial results of the splits that a row's keys reach, joined in their order: weights 2^(m_z - max m), fp32.
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
-  const int t = blockIdx.x, lane = threadIdx.x & 63;
+// ---- many rows of wide heads (256, 512 columns): one workgroup (4 waves, 64 rows) per (kv head, tile of rows, split of the keys) -------------------------------
+// A row of O does not fit one wave's registers next to another 31 of them, so the head's columns are shared out: of S^T = K Q^T (32 keys, 32 x 32 x 16 products) wave w
+// takes 32 rows (w % 2) and half of the columns (w / 2), the scores pass through LDS, and of O^T wave w has a quarter of the columns for all 64 rows.
+// Maximum and sum of a row are kept by every wave, as in the kernel for few rows, and follow as in the one for many.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_attn_wide_kernel(AttnArgs a) {
+  constexpr int BN = 32, BM = 64, ROWB = HD * 2, TILEB = BN * ROWB, DS = HD / 32, DT = HD / 128;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V], scores
+  f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [4 waves][4][64 lanes]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
+  Work w;
+  if (!find_work(a, BM, lane, w)) return;
+  const int first = row_pos(w, w.row0, a.grp), last = row_pos(w, min(w.row0 + BM, w.rows) - 1, a.grp);
+  int pos[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) { const int row = w.row0 + b * 32 + c32; pos[b] = row < w.rows ? row_pos(w, row, a.grp) : -1; }
+  bf16x8_t qf[DS];
+  const int qrow = w.row0 + (wave & 1) * 32 + c32, qcol = (wave >> 1) * (HD / 2) + half * 8;
+  {
+    const int row = min(qrow, w.rows - 1), tok = row / a.grp;
+    const bf16_t* p = a.q + (size_t)(w.t0 + tok) * a.ldq + (size_t)(w.hk * a.grp + row - tok * a.grp) * a.hd;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) qf[s] = *(const bf16x8_t*)(p + (qcol + s * 16 < a.hd ? qcol + s * 16 : 0));
+  }
+  f32x16_t o[2][DT];
+  float m[2], l[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    m[b] = -INFINITY; l[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[b][d][e] = 0.f;
+  }
+  const int krow = c32 * ROWB, kswz = swz32<HD>(c32), kc0 = (wave >> 1) * (HD / 16) + half;
+  const int vr = 4 * half + ((lane & 15) >> 2), vc = (lane & 16) + (lane & 3) * 4;
+  const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((wave * (HD / 32) + (vc >> 3)) ^ swz32<HD>(vr)) << 4) + (vc & 7) * 2;
+
+  Copier<HD, BN, swz32<HD>> cp;
+  cp.init(a, wave, lane);
+  cp.pages(a, w, w.k0, wave);
+  if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
+  cp.pages(a, w, w.k0 + BN, wave);
+#pragma unroll
+  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], qrow < w.rows && qcol + s * 16 < a.hd);
+  find_gap(a, lane, w);
+  int stage = 0;
+  for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one and with the scores
+    if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
+    const char* kt = smem + stage * 2 * TILEB;
+    {
+      f32x16_t s;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < DS; ++q) s = mfma32(*(const bf16x8_t*)(kt + krow + (((kc0 + 2 * q) ^ kswz) << 4)), qf[q], s);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sx[(wave * 4 + e) * 64 + lane] = (f32x4_t){s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]};
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const bool hide = w.gap || j0 + BN - 1 > first, uneven = first < last && j0 + BN - 1 > first;
+    uint32_t seen[2] = {0xffffu, 0xffffu};                     // bit e: key 8 (e / 4) + 4 half + e % 4
+    bf16x8_t pf[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x4_t p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p[e] = sx[(b * 4 + e) * 64 + lane] + sx[((b + 2) * 4 + e) * 64 + lane];
+      if (hide) {
+        seen[b] = 0;
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int j = j0 + e4 * 8 + half * 4;
+          const bool there = page_there(a, w, j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool see = there && j + e <= pos[b] && j + e < w.k1;
+            p[e4][e] = see ? p[e4][e] : -INFINITY;
+            seen[b] |= (uint32_t)see << (e4 * 4 + e);
+          }
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fmaxf(p[e][0], p[e][1]), fmaxf(p[e][2], p[e][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2;
+      if (__any(mx > m[b] + 8.f)) {
+        const float mn = fmaxf(m[b], mx), ms = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(m[b] - ms);
+        m[b] = mn;
+        l[b] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[b][d] *= f;
+      }
+      const float ms = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { p[e4][e] = __builtin_amdgcn_exp2f(fmaf(p[e4][e], a.scale_log2, -ms)); l[b] += p[e4][e]; }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        pf[b][t] = __builtin_bit_cast(bf16x8_t, (u32x4_t){pack2bf(p[2 * t][0], p[2 * t][1]), pack2bf(p[2 * t][2], p[2 * t][3]), pack2bf(p[2 * t + 1][0], p[2 * t + 1][1]),
+                                                          pack2bf(p[2 * t + 1][2], p[2 * t + 1][3])});
+    }
+    const uint32_t va = vaddr0 + stage * 2 * TILEB, vb = va ^ 32;       // rows + 8: the swizzle differs by two pieces
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      bf16x8_t vf[2];
+      const uint32_t x = va ^ (d * 64), y = vb ^ (d * 64);
+      vf[0] = tr_join(ds_read_tr_na<0>(x), ds_read_tr_na<8 * ROWB>(y));
+      vf[1] = tr_join(ds_read_tr_na<16 * ROWB>(x), ds_read_tr_na<24 * ROWB>(y));
+      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vf[0]), "+v"(vf[1])::"memory");
+      if (uneven && __any(not_finite(vf[0]) || not_finite(vf[1]))) {
+        bf16x8_t code[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) take_out(vf[t], code[t]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          f32x16_t c;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) c[e] = 0.f;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) c = mfma32(code[t], seen8(seen[b] >> (8 * t)), c);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[b][d][e] = put_back(o[b][d][e], c[e]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) o[b][d] = mfma32(vf[t], pf[b][t], o[b][d]);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const float lt = l[b] + __shfl_xor(l[b], 32, 64), inv = lt == 0.f ? 0.f : 1.f / lt;
+    const int row = w.row0 + b * 32 + c32, tok = row / a.grp;
+    if (row >= w.rows) continue;
+    const int h = w.hk * a.grp + row - tok * a.grp;
+    const size_t t = w.t0 + tok, rid = ((size_t)w.sp * a.T + t) * a.H + h;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        put_out(a, t, h, rid, wave * (HD / 4) + d * 32 + e * 8 + half * 4, (f32x4_t){o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]}, inv);
+    if (a.nsplit > 1 && wave == 0 && half == 0) { a.part_ml[rid * 2] = m[b]; a.part_ml[rid * 2 + 1] = lt; }
+  }
+}
+
+// The partial results of the splits that a row's keys reach, joined in the splits' order with weights 2^(m_z - max m) in fp32.
+// What both kernels need of a row: how many splits its keys reach.
+__device__ __forceinline__ int splits_of(const AttnArgs& a, int t, int lane) {
   const int r = __builtin_amdgcn_readfirstlane(find_stream(a.cu, a.R, t, lane));
-  if (r < 0) return;
+  if (r < 0) return -1;
   const int t0 = max(0, min(a.cu[r], a.T)), n = max(0, min(a.cu[r + 1], a.T) - t0);
   const int kv = (int)min((long)max(a.kv_lens[r], 0), (long)a.width << a.shift);
   const int pos = kv - n + (t - t0);
-  const int nz = pos < 0 ? 0 : (int)(pos / split_keys(kv, a.nsplit, a.cmin)) + 1;
+  return pos < 0 ? 0 : (int)(pos / split_keys(kv, a.nsplit, a.cmin)) + 1;
+}
+// Few splits (up to FEW_SPLITS; many rows): a thread takes four columns of a row through all of them.
+__global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
+  const int t = blockIdx.x, nz = splits_of(a, t, threadIdx.x & 63);
   const int idx = blockIdx.y * 256 + threadIdx.x;
-  if (idx >= a.H * a.hd / 4) return;
+  if (nz < 0 || idx >= a.H * a.hd / 4) return;
   const int h = idx * 4 / a.hd;
   const size_t step = (size_t)a.T * a.H, rid = (size_t)t * a.H + h;
   float mx = -INFINITY;
@@ -553,52 +667,84 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
   for (int z = 0; z < nz; ++z) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[(rid + z * step) * 2] - mx);
-    l += f * a.part_ml[(rid + z * step) * 2 + 1];
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[(rid + z * step) * 2] - mx), lz = a.part_ml[(rid + z * step) * 2 + 1];
     const f32x4_t p = *(const f32x4_t*)(a.part_o + (rid + z * step) * a.hd + (idx * 4 - h * a.hd));
-    if (f != 0.f) o += p * f;
+    if (f != 0.f) { o += p * f; l += lz * f; }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *(u32x2_t*)(a.out + (size_t)t * a.ldo + idx * 4) = (u32x2_t){pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
 }
+// Many splits (few rows): a workgroup per row, the splits taken by hd / 4 lanes each, as many at once as fit.
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
+  __shared__ float wt[MAX_SPLITS];
+  __shared__ f32x4_t sum[256];
+  const int t = blockIdx.x / a.H, h = blockIdx.x % a.H, tid = threadIdx.x, lane = tid & 63;
+  const int nz = splits_of(a, t, lane);
+  if (nz < 0) return;
+  const size_t step = (size_t)a.T * a.H, rid = (size_t)t * a.H + h;
+  float mx = -INFINITY, l = 0.f;
+  for (int z = lane; z < nz; z += 64) mx = fmaxf(mx, a.part_ml[(rid + z * step) * 2]);      // (every wave for itself)
+  mx = wave_max(mx);
+  if (mx == -INFINITY) mx = 0.f;
+  for (int z = lane; z < nz; z += 64) {
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[(rid + z * step) * 2] - mx);
+    l += f == 0.f ? 0.f : f * a.part_ml[(rid + z * step) * 2 + 1];
+    if (tid < 64) wt[z] = f;
+  }
+  l = wave_sum(l);
+  __syncthreads();
+  const int d4 = a.hd / 4, groups = 256 / d4, grp = tid / d4, c = tid - grp * d4;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  if (grp < groups)
+    for (int z = grp; z < nz; z += groups) {
+      const float f = wt[z];
+      const f32x4_t p = *(const f32x4_t*)(a.part_o + (rid + z * step) * a.hd + c * 4);
+      if (f != 0.f) o += p * f;
+    }
+  sum[tid] = o;
+  __syncthreads();
+  if (tid >= d4) return;
+  for (int i = 1; i < groups; ++i) o += sum[i * d4 + tid];
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *(u32x2_t*)(a.out + (size_t)t * a.ldo + (size_t)h * a.hd + c * 4) = (u32x2_t){pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
+}
 
 // ---- choices on the host, from sizes alone -----------------------------------------------------------------------------------------------------------
-struct Choice { int hd, nq, nsplit, cmin; long tiles; };
+struct Choice { int hd, bm, nsplit, cmin; long tiles; };
 
 Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, int cu_count) {
   Choice c;
   c.hd = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : hd <= 512 ? 512 : 1024;
   const int grp = H / Hkv;
   const long rows = (max_new > 0 && max_new < T ? max_new : (T + R - 1) / R) * grp;      // rows of a stream and kv head
-  c.nq = rows <= 16 || c.hd == 1024 ? 1 : c.hd == 512 ? 2 : c.hd == 256 ? 4 : 0;      // 0: the kernel for many rows
-  c.tiles = (long)T * grp / (c.nq ? 16 * c.nq : 128) + R;
+  c.bm = rows <= 16 || c.hd == 1024 ? 16 : c.hd <= 128 ? 128 : 64;
+  c.tiles = (long)T * grp / c.bm + R;
   c.cmin = 256;
   const long items = c.tiles * Hkv;
-  long want = (2l * cu_count + items - 1) / items, most = (max_kv + c.cmin - 1) / c.cmin;
-  if (want > most) want = most;
-  if (want > 128) want = 128;
-  c.nsplit = want < 1 ? 1 : (int)want;
+  // Enough workgroups for two on every CU, down to 256 keys each; and where the keys are many, four times that, so that streams of different lengths even out, but
+  // no fewer than 1024 keys each (a split costs its partial results and the join).
+  const long fill = std::min((2l * cu_count + items - 1) / items, (max_kv + c.cmin - 1) / c.cmin), even = std::min((8l * cu_count + items - 1) / items, max_kv / 1024);
+  c.nsplit = (int)std::max(1l, std::min(std::max(fill, even), (long)MAX_SPLITS));
   return c;
 }
 
 long part_floats(const Choice& c, long T, long H, long hd) { return c.nsplit > 1 ? c.nsplit * T * H * (hd + 2) : 0; }
 
-template <int HD, int NQ, int BN>
-int launch_tiles(const AttnArgs& a, const Choice& c, hipStream_t st) {
-  constexpr int lds = 4 * BN * HD * 2 + NQ * 4096;
-  static_assert(lds <= 160 * 1024, "LDS");
-  if constexpr (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)paged_attn_tile_kernel<HD, NQ, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+template <class F>
+int launch(F* kernel, int lds, const AttnArgs& a, const Choice& c, hipStream_t st) {
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     AVT_CHECK(e == hipSuccess, "avt_paged_attn_fwd: %s", hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((paged_attn_tile_kernel<HD, NQ, BN>), dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(256), lds, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(256), lds, st, a);
   return 0;
 }
+template <int HD, int BN>
+int launch_tiles(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_tile_kernel<HD, BN>, 4 * BN * HD * 2 + 4096, a, c, st); }
 template <int HD>
-int launch_long(const AttnArgs& a, const Choice& c, hipStream_t st) {
-  hipLaunchKernelGGL((paged_attn_long_kernel<HD>), dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(256), 4 * 64 * HD * 2, st, a);
-  return 0;
-}
+int launch_long(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_long_kernel<HD>, 4 * 64 * HD * 2, a, c, st); }
+template <int HD>
+int launch_wide(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_wide_kernel<HD>, 4 * 32 * HD * 2 + 16384, a, c, st); }
 constexpr int CUS = 256;
 }  // namespace
 
@@ -618,6 +764,7 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   AVT_CHECK(q && kcache && vcache && table && cu && kv_lens && out, "avt_paged_attn_fwd: null argument");
   AVT_CHECK(ldq >= (long)H * head_dim && ldo >= (long)H * head_dim && ldq % 8 == 0 && ldo % 8 == 0 && aligned16(q) && aligned16(kcache) && aligned16(vcache) && aligned16(out),
             "avt_paged_attn_fwd: 16-byte aligned rows required");
+  AVT_CHECK((long)Hkv * head_dim < (1l << 26), "avt_paged_attn_fwd: a token's row is too long (%d heads of %d)", Hkv, head_dim);
   AVT_CHECK((long)T * H < 0x7f000000l, "avt_paged_attn_fwd: too many rows for one call (%d tokens of %d heads)", T, H);
   const Choice c = choose(T, R, H, Hkv, head_dim, max_new, max_kv > 0 ? max_kv : 0x7fffffff, CUS);
   AVT_CHECK(c.tiles * Hkv < 0x7f000000l, "avt_paged_attn_fwd: too many rows for one call (%d tokens of %d streams)", T, R);
@@ -631,14 +778,14 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   a.q_and = scale == 0.f ? 0u : 0xffffffffu; a.q_xor = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t st = (hipStream_t)stream;
   int rc = 0;
-  if (c.nq == 1) rc = c.hd == 64 ? launch_tiles<64, 1, 64>(a, c, st) : c.hd == 128 ? launch_tiles<128, 1, 64>(a, c, st) : c.hd == 256 ? launch_tiles<256, 1, 32>(a, c, st)
-                    : c.hd == 512 ? launch_tiles<512, 1, 32>(a, c, st) : launch_tiles<1024, 1, 16>(a, c, st);
-  else rc = c.hd == 64 ? launch_long<64>(a, c, st) : c.hd == 128 ? launch_long<128>(a, c, st) : c.hd == 256 ? launch_tiles<256, 4, 32>(a, c, st)
-          : launch_tiles<512, 2, 32>(a, c, st);
+  if (c.bm == 16) rc = c.hd == 64 ? launch_tiles<64, 64>(a, c, st) : c.hd == 128 ? launch_tiles<128, 32>(a, c, st) : c.hd == 256 ? launch_tiles<256, 16>(a, c, st)
+                     : c.hd == 512 ? launch_tiles<512, 16>(a, c, st) : launch_tiles<1024, 16>(a, c, st);
+  else rc = c.hd == 64 ? launch_long<64>(a, c, st) : c.hd == 128 ? launch_long<128>(a, c, st) : c.hd == 256 ? launch_wide<256>(a, c, st) : launch_wide<512>(a, c, st);
   if (rc) return rc;
   AVT_LAUNCH_CHECK();
   if (c.nsplit > 1) {
-    hipLaunchKernelGGL(paged_attn_join_kernel, dim3(T, (H * head_dim / 4 + 255) / 256), dim3(256), 0, st, a);
+    if (c.nsplit <= FEW_SPLITS) hipLaunchKernelGGL(paged_attn_join_few_kernel, dim3(T, (H * head_dim / 4 + 255) / 256), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(paged_attn_join_kernel, dim3(T * H), dim3(256), 0, st, a);
     AVT_LAUNCH_CHECK();
   }
   return 0;
