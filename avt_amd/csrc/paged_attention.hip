@@ -118,13 +118,13 @@ __device__ __forceinline__ void find_gap(const AttnArgs& a, int lane, Work& w) {
   w.gap = __any(gap);
 }
 
-// Copies of K and V tiles of BN keys into LDS by 4 waves, 1 KB an instruction.  A wave copies a quarter of the tile's rows, which lie in one page (two, where they
+// Copies of K and V tiles of BN keys into LDS by NW waves, 1 KB an instruction.  A wave copies its share of the tile's rows, which lie in one page (two, where they
 // are 16 and a page may hold 8): the pages' addresses are scalar, and what a lane adds to them does not change from tile to tile, so a copy is little more than its own
 // instruction.  Rows behind the last key, rows of no page and columns behind the head's are asked for out of range and arrive as zeros: what is not
 // finite in memory that holds no key never meets a probability of 0.
-template <int HD, int BN, int (*SWZ)(int)>
+template <int HD, int BN, int NW, int (*SWZ)(int)>
 struct Copier {
-  static constexpr int ROWB = HD * 2, TILEB = BN * ROWB, NI = TILEB / 4096, RW = BN / 4, PG = RW > 8 ? 2 : 1, RP = RW / PG;      // rows of a wave, of a page's part
+  static constexpr int ROWB = HD * 2, TILEB = BN * ROWB, NI = TILEB / 1024 / NW, RW = BN / NW, PG = RW > 8 ? 2 : 1, RP = RW / PG;      // rows of a wave, of a page's part
   static constexpr uint32_t NONE = 0xFFFFFFF0u;
   uint32_t off[NI];                                            // of the lane's 16 bytes from its part's first row
   int pg[PG];
@@ -150,8 +150,8 @@ struct Copier {
       for (int i = q * NI / PG; i < (q + 1) * NI / PG; ++i) {
         uint32_t v = off[i];
         if (!whole && (jb + (i * 1024 + lane * 16) / ROWB % RP >= w.k1 || !there)) v = NONE;
-        copy(a.kc + at, dst + wave * (TILEB / 4) + i * 1024, v);
-        copy(a.vc + at, dst + TILEB + wave * (TILEB / 4) + i * 1024, v);
+        copy(a.kc + at, dst + wave * (TILEB / NW) + i * 1024, v);
+        copy(a.vc + at, dst + TILEB + wave * (TILEB / NW) + i * 1024, v);
       }
     }
   }
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
   const int vr = 4 * g + (c16 >> 2);
   const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((wave * (HD / 32) + ((c16 & 3) >> 1)) ^ swz16<HD>(vr)) << 4) + (c16 & 1) * 8;
 
-  Copier<HD, BN, swz16<HD>> cp;
+  Copier<HD, BN, 4, swz16<HD>> cp;
   cp.init(a, wave, lane);
   cp.pages(a, w, w.k0, wave);
   if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
   const int vc = (lane & 16) + (lane & 3) * 4;
   const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((vc >> 3) ^ swz32<HD>(vr)) << 4) + (vc & 7) * 2;
 
-  Copier<HD, BN, swz32<HD>> cp;
+  Copier<HD, BN, 4, swz32<HD>> cp;
   cp.init(a, wave, lane);
   cp.pages(a, w, w.k0, wave);
   if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
@@ -402,15 +402,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
     const char* kt = smem + stage * 2 * TILEB;
     f32x16_t s[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[k][e] = 0.f;
+    for (int q = 0; q < DS; ++q)
 #pragma unroll
-      for (int q = 0; q < DS; ++q) {
-        const bf16x8_t kf = *(const bf16x8_t*)(kt + k * 32 * ROWB + krow + (((2 * q + half) ^ kswz) << 4));
-        s[k] = mfma32(kf, qf[q], s[k]);
-      }
-    }
+      for (int k = 0; k < 2; ++k) s[k] = mfma32(*(const bf16x8_t*)(kt + k * 32 * ROWB + krow + (((2 * q + half) ^ kswz) << 4)), qf[q], s[k]);
     uint32_t seen = 0xffffffffu;                               // bit 16 k + e: key 32 k + 8 (e / 4) + 4 half + e % 4
     if (w.gap || j0 + BN - 1 > first) {
       seen = 0;
@@ -495,45 +491,48 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
   if (a.nsplit > 1 && half == 0) { a.part_ml[rid * 2] = m; a.part_ml[rid * 2 + 1] = l; }
 }
 
-// ---- many rows of wide heads (256, 512 columns): one workgroup (4 waves, 64 rows) per (kv head, tile of rows, split of the keys) -------------------------------
-// A row of O does not fit one wave's registers next to another 31 of them, so the head's columns are shared out: of S^T = K Q^T (32 keys, 32 x 32 x 16 products) wave w
-// takes 32 rows (w % 2) and half of the columns (w / 2), the scores pass through LDS, and of O^T wave w has a quarter of the columns for all 64 rows.
-// Maximum and sum of a row are kept by every wave, as in the kernel for few rows, and follow as in the one for many.
-template <int HD>
-__global__ __launch_bounds__(256) void paged_attn_wide_kernel(AttnArgs a) {
-  constexpr int BN = 32, BM = 64, ROWB = HD * 2, TILEB = BN * ROWB, DS = HD / 32, DT = HD / 128;
+// ---- many rows of wide heads (256, 512 columns): one workgroup (NW = 4 or 8 waves, 64 rows) per (kv head, tile of rows, split of the keys) --------------------
+// 32 rows of O do not fit one wave's registers, so the head's columns are shared out: of S^T = K Q^T (32 keys, 32 x 32 x 16 products) wave w takes 32 rows (w % 2) and
+// one of NW / 2 parts of the columns, the scores pass through LDS, and of O^T a wave has a quarter of the columns, for all 64 rows (4 waves, 256 columns: two
+// workgroups on a CU) or for 32 (8 waves, 512 columns: the LDS holds one).  Either way 2 waves share a SIMD and no accumulator leaves the 256 registers that
+// the vector unit reaches (with 4 waves for 512 columns the compiler kept O in the others and moved it to and fro: 8 us a tile of 32 keys).
+// Maximum and sum of a row are kept by every wave that has a part of it, as in the kernel for few rows, and follow as in the one for many.
+template <int HD, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a) {
+  constexpr int BN = 32, BM = 64, ROWB = HD * 2, TILEB = BN * ROWB, DQ = NW / 2, DS = HD / DQ / 16, DT = HD / 128, NB = 8 / NW;      // NB: row blocks of a wave's O
   extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V], scores
-  f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [4 waves][4][64 lanes]
+  f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [NW][4][64 lanes]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
+  const int slice = NB == 2 ? wave : wave >> 1, b0 = NB == 2 ? 0 : wave & 1;      // of O: quarter of the columns, first row block
   Work w;
   if (!find_work(a, BM, lane, w)) return;
   const int first = row_pos(w, w.row0, a.grp), last = row_pos(w, min(w.row0 + BM, w.rows) - 1, a.grp);
-  int pos[2];
+  int pos[NB];
 #pragma unroll
-  for (int b = 0; b < 2; ++b) { const int row = w.row0 + b * 32 + c32; pos[b] = row < w.rows ? row_pos(w, row, a.grp) : -1; }
+  for (int b = 0; b < NB; ++b) { const int row = w.row0 + (b0 + b) * 32 + c32; pos[b] = row < w.rows ? row_pos(w, row, a.grp) : -1; }
   bf16x8_t qf[DS];
-  const int qrow = w.row0 + (wave & 1) * 32 + c32, qcol = (wave >> 1) * (HD / 2) + half * 8;
+  const int qrow = w.row0 + (wave & 1) * 32 + c32, qcol = (wave >> 1) * (HD / DQ) + half * 8;
   {
     const int row = min(qrow, w.rows - 1), tok = row / a.grp;
     const bf16_t* p = a.q + (size_t)(w.t0 + tok) * a.ldq + (size_t)(w.hk * a.grp + row - tok * a.grp) * a.hd;
 #pragma unroll
     for (int s = 0; s < DS; ++s) qf[s] = *(const bf16x8_t*)(p + (qcol + s * 16 < a.hd ? qcol + s * 16 : 0));
   }
-  f32x16_t o[2][DT];
-  float m[2], l[2];
+  f32x16_t o[NB][DT];
+  float m[NB], l[NB];
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
+  for (int b = 0; b < NB; ++b) {
     m[b] = -INFINITY; l[b] = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[b][d][e] = 0.f;
   }
-  const int krow = c32 * ROWB, kswz = swz32<HD>(c32), kc0 = (wave >> 1) * (HD / 16) + half;
+  const int krow = c32 * ROWB, kswz = swz32<HD>(c32), kc0 = (wave >> 1) * (HD / DQ / 8) + half;
   const int vr = 4 * half + ((lane & 15) >> 2), vc = (lane & 16) + (lane & 3) * 4;
-  const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((wave * (HD / 32) + (vc >> 3)) ^ swz32<HD>(vr)) << 4) + (vc & 7) * 2;
+  const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((slice * (HD / 32) + (vc >> 3)) ^ swz32<HD>(vr)) << 4) + (vc & 7) * 2;
 
-  Copier<HD, BN, swz32<HD>> cp;
+  Copier<HD, BN, NW, swz32<HD>> cp;
   cp.init(a, wave, lane);
   cp.pages(a, w, w.k0, wave);
   if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
@@ -547,23 +546,32 @@ __global__ __launch_bounds__(256) void paged_attn_wide_kernel(AttnArgs a) {
     if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
     const char* kt = smem + stage * 2 * TILEB;
     {
-      f32x16_t s;
+      f32x16_t s, s1;                                          // (two chains: a product that waits for the one before it would idle the unit half of the time)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = 0.f;
+      for (int e = 0; e < 16; ++e) s[e] = s1[e] = 0.f;
 #pragma unroll
-      for (int q = 0; q < DS; ++q) s = mfma32(*(const bf16x8_t*)(kt + krow + (((kc0 + 2 * q) ^ kswz) << 4)), qf[q], s);
+      for (int q = 0; q < DS; q += 2) {
+        s = mfma32(*(const bf16x8_t*)(kt + krow + (((kc0 + 2 * q) ^ kswz) << 4)), qf[q], s);
+        s1 = mfma32(*(const bf16x8_t*)(kt + krow + (((kc0 + 2 * q + 2) ^ kswz) << 4)), qf[q + 1], s1);
+      }
+      s += s1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) sx[(wave * 4 + e) * 64 + lane] = (f32x4_t){s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]};
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const bool hide = w.gap || j0 + BN - 1 > first, uneven = first < last && j0 + BN - 1 > first;
-    uint32_t seen[2] = {0xffffu, 0xffffu};                     // bit e: key 8 (e / 4) + 4 half + e % 4
-    bf16x8_t pf[2][2];
+    uint32_t seen[NB];                                         // bit e: key 8 (e / 4) + 4 half + e % 4
+    bf16x8_t pf[NB][2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < NB; ++b) {
       f32x4_t p[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = sx[(b * 4 + e) * 64 + lane] + sx[((b + 2) * 4 + e) * 64 + lane];
+      for (int e = 0; e < 4; ++e) {
+        p[e] = sx[((b0 + b) * 4 + e) * 64 + lane];
+#pragma unroll
+        for (int q = 1; q < DQ; ++q) p[e] += sx[((2 * q + b0 + b) * 4 + e) * 64 + lane];
+      }
+      seen[b] = 0xffffu;
       if (hide) {
         seen[b] = 0;
 #pragma unroll
@@ -600,38 +608,48 @@ __global__ __launch_bounds__(256) void paged_attn_wide_kernel(AttnArgs a) {
                                                           pack2bf(p[2 * t + 1][2], p[2 * t + 1][3])});
     }
     const uint32_t va = vaddr0 + stage * 2 * TILEB, vb = va ^ 32;       // rows + 8: the swizzle differs by two pieces
+    constexpr int G = NB == 2 ? 1 : 2;                         // column blocks whose fragments are read at once
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      bf16x8_t vf[2];
-      const uint32_t x = va ^ (d * 64), y = vb ^ (d * 64);
-      vf[0] = tr_join(ds_read_tr_na<0>(x), ds_read_tr_na<8 * ROWB>(y));
-      vf[1] = tr_join(ds_read_tr_na<16 * ROWB>(x), ds_read_tr_na<24 * ROWB>(y));
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vf[0]), "+v"(vf[1])::"memory");
-      if (uneven && __any(not_finite(vf[0]) || not_finite(vf[1]))) {
-        bf16x8_t code[2];
+    for (int d0 = 0; d0 < DT; d0 += G) {
+      bf16x8_t vf[G][2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) take_out(vf[t], code[t]);
+      for (int d = 0; d < G; ++d) {
+        const uint32_t x = va ^ ((d0 + d) * 64), y = vb ^ ((d0 + d) * 64);
+        vf[d][0] = tr_join(ds_read_tr_na<0>(x), ds_read_tr_na<8 * ROWB>(y));
+        vf[d][1] = tr_join(ds_read_tr_na<16 * ROWB>(x), ds_read_tr_na<24 * ROWB>(y));
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          f32x16_t c;
+      for (int d = 0; d < G; ++d) {
+        asm volatile("" : "+v"(vf[d][0]), "+v"(vf[d][1]));
+        if (uneven && __any(not_finite(vf[d][0]) || not_finite(vf[d][1]))) {
+          bf16x8_t code[2];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) c[e] = 0.f;
+          for (int t = 0; t < 2; ++t) take_out(vf[d][t], code[t]);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) c = mfma32(code[t], seen8(seen[b] >> (8 * t)), c);
+          for (int b = 0; b < NB; ++b) {
+            f32x16_t c;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[b][d][e] = put_back(o[b][d][e], c[e]);
+            for (int e = 0; e < 16; ++e) c[e] = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) c = mfma32(code[t], seen8(seen[b] >> (8 * t)), c);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[b][d0 + d][e] = put_back(o[b][d0 + d][e], c[e]);
+          }
         }
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) o[b][d] = mfma32(vf[t], pf[b][t], o[b][d]);
+        for (int d = 0; d < G; ++d)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) o[b][d0 + d] = mfma32(vf[d][t], pf[b][t], o[b][d0 + d]);
     }
   }
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
+  for (int b = 0; b < NB; ++b) {
     const float lt = l[b] + __shfl_xor(l[b], 32, 64), inv = lt == 0.f ? 0.f : 1.f / lt;
-    const int row = w.row0 + b * 32 + c32, tok = row / a.grp;
+    const int row = w.row0 + (b0 + b) * 32 + c32, tok = row / a.grp;
     if (row >= w.rows) continue;
     const int h = w.hk * a.grp + row - tok * a.grp;
     const size_t t = w.t0 + tok, rid = ((size_t)w.sp * a.T + t) * a.H + h;
@@ -639,8 +657,8 @@ __global__ __launch_bounds__(256) void paged_attn_wide_kernel(AttnArgs a) {
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        put_out(a, t, h, rid, wave * (HD / 4) + d * 32 + e * 8 + half * 4, (f32x4_t){o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]}, inv);
-    if (a.nsplit > 1 && wave == 0 && half == 0) { a.part_ml[rid * 2] = m[b]; a.part_ml[rid * 2 + 1] = lt; }
+        put_out(a, t, h, rid, slice * (HD / 4) + d * 32 + e * 8 + half * 4, (f32x4_t){o[b][d][4 * e], o[b][d][4 * e + 1], o[b][d][4 * e + 2], o[b][d][4 * e + 3]}, inv);
+    if (a.nsplit > 1 && slice == 0 && half == 0) { a.part_ml[rid * 2] = m[b]; a.part_ml[rid * 2 + 1] = lt; }
   }
 }
 
@@ -731,20 +749,20 @@ Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, i
 long part_floats(const Choice& c, long T, long H, long hd) { return c.nsplit > 1 ? c.nsplit * T * H * (hd + 2) : 0; }
 
 template <class F>
-int launch(F* kernel, int lds, const AttnArgs& a, const Choice& c, hipStream_t st) {
+int launch(F* kernel, int threads, int lds, const AttnArgs& a, const Choice& c, hipStream_t st) {
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     AVT_CHECK(e == hipSuccess, "avt_paged_attn_fwd: %s", hipGetErrorString(e));
   }
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(256), lds, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(c.tiles * a.Hkv), c.nsplit), dim3(threads), lds, st, a);
   return 0;
 }
 template <int HD, int BN>
-int launch_tiles(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_tile_kernel<HD, BN>, 4 * BN * HD * 2 + 4096, a, c, st); }
+int launch_tiles(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_tile_kernel<HD, BN>, 256, 4 * BN * HD * 2 + 4096, a, c, st); }
 template <int HD>
-int launch_long(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_long_kernel<HD>, 4 * 64 * HD * 2, a, c, st); }
-template <int HD>
-int launch_wide(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_wide_kernel<HD>, 4 * 32 * HD * 2 + 16384, a, c, st); }
+int launch_long(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_long_kernel<HD>, 256, 4 * 64 * HD * 2, a, c, st); }
+template <int HD, int NW>
+int launch_wide(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_wide_kernel<HD, NW>, NW * 64, 4 * 32 * HD * 2 + NW * 4096, a, c, st); }
 constexpr int CUS = 256;
 }  // namespace
 
@@ -780,7 +798,7 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   int rc = 0;
   if (c.bm == 16) rc = c.hd == 64 ? launch_tiles<64, 64>(a, c, st) : c.hd == 128 ? launch_tiles<128, 32>(a, c, st) : c.hd == 256 ? launch_tiles<256, 16>(a, c, st)
                      : c.hd == 512 ? launch_tiles<512, 16>(a, c, st) : launch_tiles<1024, 16>(a, c, st);
-  else rc = c.hd == 64 ? launch_long<64>(a, c, st) : c.hd == 128 ? launch_long<128>(a, c, st) : c.hd == 256 ? launch_wide<256>(a, c, st) : launch_wide<512>(a, c, st);
+  else rc = c.hd == 64 ? launch_long<64>(a, c, st) : c.hd == 128 ? launch_long<128>(a, c, st) : c.hd == 256 ? launch_wide<256, 4>(a, c, st) : launch_wide<512, 8>(a, c, st);
   if (rc) return rc;
   AVT_LAUNCH_CHECK();
   if (c.nsplit > 1) {
