@@ -740,8 +740,8 @@ Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, i
   c.cmin = 256;
   const long items = c.tiles * Hkv;
   // Enough workgroups for two on every CU, down to 256 keys each; and where the keys are many, four times that, so that streams of different lengths even out, but
-  // no fewer than 1024 keys each (a split costs its partial results and the join).
-  const long fill = std::min((2l * cu_count + items - 1) / items, (max_kv + c.cmin - 1) / c.cmin), even = std::min((8l * cu_count + items - 1) / items, max_kv / 1024);
+  // no fewer than 1024 keys each (a split costs its partial results and the join: with many rows those are as much as the keys, 403 against 440 us without it).
+  const long fill = std::min((2l * cu_count + items - 1) / items, (max_kv + c.cmin - 1) / c.cmin), even = std::min((8l * cu_count + items - 1) / items, c.bm > 16 ? 0l : max_kv / 1024);
   c.nsplit = (int)std::max(1l, std::min(std::max(fill, even), (long)MAX_SPLITS));
   return c;
 }
