@@ -143,6 +143,11 @@ class AVTh(nn.Module):
         dec, last = _HeadFn.apply(self, arena, keep, self.training, seed, feats, self.encoder.weight, extra, group or _NodeGroup(1))
         return dec if (extra is None and group is None) else (dec, last)
 
+    def open_streams(self, streams, **kw):
+        """``streams`` live clips of different lengths on this head (avt_amd/models/streams.py): append frames as they come, roll out from where each clip is."""
+        from .streams import HeadStreams
+        return HeadStreams(self, streams, **kw)
+
     def _rollout(self, feats, output_len):
         arena = get_arena(self)
         arena.refresh_shadow()

@@ -8,9 +8,13 @@ Tolerances.  u = eps(bf16) / 2 = 2^-8 is the half step of the output's rounding 
   w4          |y - ref| <= u |ref| + K 2^-23 B,  B = sum |x| s |u - 8| + the offset's part 24 sum |x| s (K additions of half steps 2^-24, twice for offset and groups);
               the tanh GELU's slope is at most 1.13 and its own error below 2^-18 of its argument."""
 import math
+import os
+import sys
 
 import pytest
 import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
 from avt_amd.lib import AvtHipError
 
@@ -489,3 +493,118 @@ def test_w4_refuses_and_takes_nothing(ops):
                  (torch.zeros((8, 64), dtype=torch.uint8), torch.zeros((8, 1))), (torch.zeros((8, 256), dtype=torch.uint8), torch.zeros((8, 2), dtype=BF16))):
         with pytest.raises(AvtHipError):
             ops.W4Weight(q.cuda(), s.cuda())
+
+
+# ---- a run of them together: the head's streams ------------------------------------------------------------------------------------------------
+def build_head(in_dim, inter, layers, heads, seed=0):
+    """(the head on the GPU, the oracle's with the same weights)."""
+    from helpers import build_hip_model, build_oracle_model
+    torch.manual_seed(seed)
+    orc = build_oracle_model('feat', in_dim, inter, layers, heads, 11).future_predictor
+    with torch.no_grad():
+        for p in orc.parameters():
+            if p.ndim >= 2:
+                p.normal_(0, 0.6 * p.size(-1) ** -0.5)
+    model = build_hip_model('feat', in_dim, inter, layers, heads, 11).eval()
+    model.future_predictor.load_state_dict(orc.state_dict())
+    return model.future_predictor, orc.eval()
+
+
+def oracle_decode(orc, clip, steps):
+    """The oracle's decoded features of a clip (T, C) and of a roll-out of `steps` from its end: (T - 1 + steps, C)."""
+    with torch.no_grad():
+        orc.output_len = orc.output_len_eval = steps
+        orc.avg_last_n, orc.return_past_too = -1, False
+        past, future, _, _ = orc(clip[None], (1, steps, clip.size(1)))
+    return torch.cat([past[0, 1:], future[0]], 0)
+
+
+TOL = 3e-2      # of the largest magnitude: the head's own limit against the fp32 oracle (bf16 activations and weights in every product)
+
+
+def close(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    assert float((a - b).abs().max()) <= TOL * float(b.abs().max()), float((a - b).abs().max() / b.abs().max())
+
+
+@pytest.mark.parametrize('in_dim,inter,layers,heads,page', [(64, 64, 2, 2, 8), (128, 256, 2, 1, 16), (768, 2048, 6, 4, 16)])
+def test_streams_of_different_lengths_match_the_oracle(ops, in_dim, inter, layers, heads, page):
+    """Frames come in chunks of every size; each stream decodes what the oracle decodes of its clip alone, and rolls out as it does."""
+    head, orc = build_head(in_dim, inter, layers, heads)
+    g = torch.Generator().manual_seed(1)
+    total = [5, 0, 20, 13, 1]
+    clips = [torch.randn((t, in_dim), generator=g) for t in total]
+    st = head.open_streams(5, max_len=30, page=page)
+    seen, got = [0] * 5, [[] for _ in range(5)]
+    for counts in ([2, 0, 11, 1, 0], [0, 0, 0, 0, 0], [1, 0, 8, 9, 0], [2, 0, 1, 3, 1]):
+        feats = torch.cat([c[s:s + n] for c, s, n in zip(clips, seen, counts)])
+        out = st.append(feats.cuda(), counts)
+        for s, part in enumerate(out.split(counts)):
+            got[s].append(part)
+        seen = [a + b for a, b in zip(seen, counts)]
+    assert st.lengths == total == seen
+    fut = st.rollout(4)
+    again = st.rollout(4)                                      # the streams are as they were
+    assert torch.equal(fut, again) and not fut[1].any()
+    for s, t in enumerate(total):
+        if t:
+            want = oracle_decode(orc, clips[s], 4)
+            close(torch.cat(got[s]), want[:t])
+            close(fut[s], want[t - 1:])
+    more = torch.randn((3, in_dim), generator=g)               # and go on from their frames, not from what was rolled out
+    out = st.append(more.cuda(), [3, 0, 0, 0, 0])
+    close(out, oracle_decode(orc, torch.cat([clips[0], more]), 1)[5:])
+
+
+def test_streams_release_and_refuse(ops):
+    head, orc = build_head(64, 64, 2, 2)
+    st = head.open_streams(3, max_len=40, page=8, pages=7)
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((40, 64), generator=g)
+    first = st.append(x[:30].cuda(), [20, 10, 0])              # 3 + 2 pages
+    with pytest.raises(ValueError, match='pages short'):
+        st.append(x[:17].cuda(), [0, 0, 17])                   # 3 more: 2 are there
+    with pytest.raises(ValueError, match='more than its 40'):
+        st.append(x[:21].cuda(), [21, 0, 0])
+    with pytest.raises(ValueError, match='more than its 40'):
+        st.rollout(22)
+    for feats, counts in ((x[:3].cuda(), [1, 1]), (x[:3].cuda(), [1, 1, 2]), (x[:3].cuda(), [4, -1, 0]), (x[:3, :32].cuda(), [1, 1, 1])):
+        with pytest.raises(ValueError):
+            st.append(feats, counts)
+    assert st.lengths == [20, 10, 0]                           # what was refused left nothing behind
+    st.release([0, 0])
+    assert st.lengths == [0, 10, 0] and int(st.n_free) == 5
+    out = st.append(torch.cat([x[:17], x[20:21]]).cuda(), [17, 1, 0])      # stream 0 is another clip now, on used pages
+    close(out[:17], oracle_decode(orc, x[:17], 1))
+    close(out[17:], oracle_decode(orc, torch.cat([x[20:30], x[20:21]]), 1)[10:])
+    close(out[:17], first[:17])
+    for kw in (dict(page=12), dict(max_len=0), dict(max_len=5000), dict(weight_bits=8), dict(pages=0)):
+        with pytest.raises(ValueError):
+            head.open_streams(2, **kw)
+
+
+def test_streams_on_four_bit_weights(ops):
+    """The same as a head whose projections hold the values that the 4-bit weights stand for."""
+    head, _ = build_head(128, 256, 3, 2)
+    st4 = head.open_streams(2, max_len=64, weight_bits=4)
+    from avt_amd.models.streams import HeadStreams
+    with torch.no_grad():
+        for b in head.gpt_model.h:
+            for lin in (b.attn.c_attn, b.attn.c_proj, b.mlp.c_fc, b.mlp.c_proj):
+                lin.weight.copy_(HeadStreams._quantize(lin.weight).dequantize().t())
+    st = head.open_streams(2, max_len=64)
+    x = torch.randn((40, 128), generator=torch.Generator().manual_seed(4)).cuda()
+    for lo, counts in ((0, [20, 5]), (25, [1, 1]), (27, [0, 13])):
+        f = x[lo:lo + sum(counts)]
+        close(st4.append(f, counts), st.append(f, counts))
+    close(st4.rollout(3), st.rollout(3))
+
+
+def test_streams_go_past_the_contiguous_cache_kernels_limits(ops):
+    """A clip of 600 frames in chunks of 100 decodes as in one of 600 (the head's own attention takes 32 frames)."""
+    head, _ = build_head(64, 128, 2, 2)
+    x = torch.randn((600, 64), generator=torch.Generator().manual_seed(6)).cuda()
+    a, b = head.open_streams(1), head.open_streams(1, page=64)
+    parts = torch.cat([a.append(x[i:i + 100], [100]) for i in range(0, 600, 100)])
+    close(parts, b.append(x, [600]))
+    close(a.rollout(5), b.rollout(5))
