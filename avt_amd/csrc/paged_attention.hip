@@ -31,10 +31,10 @@ struct AttnArgs {
   uint32_t q_and, q_xor;                                       // applied to q as it is read: the sign of a negative scale; a scale of 0 is a q of 0
 };
 
-// Keys of one split: a stream's cached tokens are cut into at most nsplit pieces, each a multiple of `cmin` keys (itself a multiple of the tile's).
+// Keys of one split: a stream's cached tokens are cut into at most nsplit pieces of at least `cmin` keys, in steps of 64 (a multiple of every tile).
 __device__ __forceinline__ long split_keys(int kv, int nsplit, int cmin) {
   const long c = ((long)kv + nsplit - 1) / nsplit;
-  return (c + cmin - 1) / cmin * cmin;
+  return ((c < cmin ? cmin : c) + 63) / 64 * 64;
 }
 
 typedef const __attribute__((address_space(4))) int* table_t;  // (the table does not change while a kernel runs: its entries come through the scalar cache)
@@ -139,6 +139,8 @@ struct Copier {
 #pragma unroll
     for (int q = 0; q < PG; ++q) pg[q] = w.tab[max(0, min(j0 + wave * RW + q * RP, w.k1 - 1)) >> a.shift];
   }
+  // K: to dst, V: to dst + TILEB; WHICH: 1 K, 2 V, 3 both
+  template <int WHICH>
   __device__ __forceinline__ void issue(const AttnArgs& a, const Work& w, int j0, char* dst, int wave, int lane) {
     const bool whole = j0 + BN <= w.k1 && !w.gap;
 #pragma unroll
@@ -150,8 +152,8 @@ struct Copier {
       for (int i = q * NI / PG; i < (q + 1) * NI / PG; ++i) {
         uint32_t v = off[i];
         if (!whole && (jb + (i * 1024 + lane * 16) / ROWB % RP >= w.k1 || !there)) v = NONE;
-        copy(a.kc + at, dst + wave * (TILEB / NW) + i * 1024, v);
-        copy(a.vc + at, dst + TILEB + wave * (TILEB / NW) + i * 1024, v);
+        if constexpr (WHICH & 1) copy(a.kc + at, dst + wave * (TILEB / NW) + i * 1024, v);
+        if constexpr (WHICH & 2) copy(a.vc + at, dst + TILEB + wave * (TILEB / NW) + i * 1024, v);
       }
     }
   }
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
   Copier<HD, BN, 4, swz16<HD>> cp;
   cp.init(a, wave, lane);
   cp.pages(a, w, w.k0, wave);
-  if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
+  if (w.k0 < w.k1) cp.template issue<3>(a, w, w.k0, smem, wave, lane);
   cp.pages(a, w, w.k0 + BN, wave);
   // (Q is waited for here: left to the first product, the compiler's wait for it would sit inside the loop and wait for the copies in flight as well)
 #pragma unroll
@@ -257,7 +259,7 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
   int stage = 0;
   for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one and with the scores
-    if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
+    if (j0 + BN < w.k1) { cp.template issue<3>(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
     const char* kt = smem + stage * 2 * TILEB;
     f32x4_t s4 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -389,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
   Copier<HD, BN, 4, swz32<HD>> cp;
   cp.init(a, wave, lane);
   cp.pages(a, w, w.k0, wave);
-  if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
+  if (w.k0 < w.k1) cp.template issue<3>(a, w, w.k0, smem, wave, lane);
   cp.pages(a, w, w.k0 + BN, wave);
 #pragma unroll
   for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], ok && s * 16 + half * 8 < a.hd);
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
   int stage = 0;
   for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one
-    if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
+    if (j0 + BN < w.k1) { cp.template issue<3>(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
     if (j0 > last) continue;                                   // none of this wave's rows sees the tile
     const char* kt = smem + stage * 2 * TILEB;
     f32x16_t s[2];
@@ -492,18 +494,20 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
 }
 
 // ---- many rows of wide heads (256, 512 columns): one workgroup (NW = 4 or 8 waves, 64 rows) per (kv head, tile of rows, split of the keys) --------------------
-// 32 rows of O do not fit one wave's registers, so the head's columns are shared out: of S^T = K Q^T (32 keys, 32 x 32 x 16 products) wave w takes 32 rows (w % 2) and
-// one of NW / 2 parts of the columns, the scores pass through LDS, and of O^T a wave has a quarter of the columns, for all 64 rows (4 waves, 256 columns: two
-// workgroups on a CU) or for 32 (8 waves, 512 columns: the LDS holds one).  Either way 2 waves share a SIMD and no accumulator leaves the 256 registers that
-// the vector unit reaches (with 4 waves for 512 columns the compiler kept O in the others and moved it to and fro: 8 us a tile of 32 keys).
+// 32 rows of O do not fit one wave's registers, so S^T and O^T are shared out in different ways.  Of S^T = K Q^T (32 keys) a wave has blocks of 16 keys x 16 rows,
+// over all of the head's columns (16 x 16 x 32 products: no partial sums to add), which pass through LDS; of O^T it has a quarter of the columns, for all 64 rows
+// (4 waves, 256 columns: two workgroups on a CU) or for 32 (8 waves, 512 columns: the LDS holds one).  Either way 2 waves share a SIMD and no accumulator leaves
+// the 256 registers that the vector unit reaches (with 4 waves for 512 columns the compiler kept O in the others and moved it to and fro: 8 us a tile).
+// The scores of tile i + 1 are made between the same two barriers as the softmax and the products with V of tile i, so that neither unit waits for the other.
 // Maximum and sum of a row are kept by every wave that has a part of it, as in the kernel for few rows, and follow as in the one for many.
 template <int HD, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a) {
-  constexpr int BN = 32, BM = 64, ROWB = HD * 2, TILEB = BN * ROWB, DQ = NW / 2, DS = HD / DQ / 16, DT = HD / 128, NB = 8 / NW;      // NB: row blocks of a wave's O
-  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V], scores
-  f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [NW][4][64 lanes]
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c32 = lane & 31, half = lane >> 5;
+  constexpr int BN = 32, BM = 64, ROWB = HD * 2, TILEB = BN * ROWB, DS = HD / 32, KB = 8 / NW, DT = HD / 128, NB = 8 / NW;      // KB: key blocks of a wave's S, NB: row blocks of its O
+  extern __shared__ __attribute__((aligned(1024))) char smem[];          // [2 tiles][K | V], scores of two tiles
+  f32x4_t* sx = (f32x4_t*)(smem + 4 * TILEB);                  // [2][2 key blocks][4 row blocks][64 lanes]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g16 = lane >> 4, c32 = lane & 31, half = lane >> 5;
   const int slice = NB == 2 ? wave : wave >> 1, b0 = NB == 2 ? 0 : wave & 1;      // of O: quarter of the columns, first row block
+  const int rb = wave & 3, kb0 = KB == 2 ? 0 : wave >> 2;      // of S: row block, first key block
   Work w;
   if (!find_work(a, BM, lane, w)) return;
   const int first = row_pos(w, w.row0, a.grp), last = row_pos(w, min(w.row0 + BM, w.rows) - 1, a.grp);
@@ -511,12 +515,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
 #pragma unroll
   for (int b = 0; b < NB; ++b) { const int row = w.row0 + (b0 + b) * 32 + c32; pos[b] = row < w.rows ? row_pos(w, row, a.grp) : -1; }
   bf16x8_t qf[DS];
-  const int qrow = w.row0 + (wave & 1) * 32 + c32, qcol = (wave >> 1) * (HD / DQ) + half * 8;
+  const int qrow = w.row0 + rb * 16 + c16;
   {
     const int row = min(qrow, w.rows - 1), tok = row / a.grp;
     const bf16_t* p = a.q + (size_t)(w.t0 + tok) * a.ldq + (size_t)(w.hk * a.grp + row - tok * a.grp) * a.hd;
 #pragma unroll
-    for (int s = 0; s < DS; ++s) qf[s] = *(const bf16x8_t*)(p + (qcol + s * 16 < a.hd ? qcol + s * 16 : 0));
+    for (int s = 0; s < DS; ++s) qf[s] = *(const bf16x8_t*)(p + (s * 32 + g16 * 8 < a.hd ? s * 32 + g16 * 8 : 0));
   }
   f32x16_t o[NB][DT];
   float m[NB], l[NB];
@@ -528,37 +532,59 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[b][d][e] = 0.f;
   }
-  const int krow = c32 * ROWB, kswz = swz32<HD>(c32), kc0 = (wave >> 1) * (HD / DQ / 8) + half;
+  const int krow = c16 * ROWB;
   const int vr = 4 * half + ((lane & 15) >> 2), vc = (lane & 16) + (lane & 3) * 4;
   const uint32_t vaddr0 = lds_addr32(smem) + TILEB + vr * ROWB + (((slice * (HD / 32) + (vc >> 3)) ^ swz32<HD>(vr)) << 4) + (vc & 7) * 2;
 
-  Copier<HD, BN, NW, swz32<HD>> cp;
-  cp.init(a, wave, lane);
-  cp.pages(a, w, w.k0, wave);
-  if (w.k0 < w.k1) cp.issue(a, w, w.k0, smem, wave, lane);
-  cp.pages(a, w, w.k0 + BN, wave);
+  const auto scores = [&](const char* kt, int which) {         // of the tile in kt, to sx
 #pragma unroll
-  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], qrow < w.rows && qcol + s * 16 < a.hd);
+    for (int k = 0; k < KB; ++k) {
+      f32x4_t s = {0.f, 0.f, 0.f, 0.f}, s1 = s;                // (two chains: a product that waits for the one before it would idle the unit half of the time)
+      const char* kr = kt + (kb0 + k) * 16 * ROWB + krow;
+      const int kswz = swz32<HD>((kb0 + k) * 16 + c16);
+#pragma unroll
+      for (int q0 = 0; q0 < DS; q0 += 8) {
+        bf16x8_t kf[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) kf[q] = *(const bf16x8_t*)(kr + (((4 * (q0 + q) + g16) ^ kswz) << 4));
+        __builtin_amdgcn_sched_barrier(0);                     // (left alone, the compiler reads two fragments ahead of the products and waits for each)
+#pragma unroll
+        for (int q = 0; q < 8; q += 2) {
+          s = mfma16(kf[q], qf[q0 + q], s);
+          s1 = mfma16(kf[q + 1], qf[q0 + q + 1], s1);
+        }
+      }
+      sx[((which * 2 + kb0 + k) * 4 + rb) * 64 + lane] = s + s1;
+    }
+  };
+  // K of tile i + 2 and V of tile i + 1 are asked for while tile i is worked on.
+  using Copy = Copier<HD, BN, NW, swz32<HD>>;
+  Copy ck, cv;
+  ck.init(a, wave, lane);
+#pragma unroll
+  for (int i = 0; i < Copy::NI; ++i) cv.off[i] = ck.off[i];
+  if (w.k0 < w.k1) {
+    ck.pages(a, w, w.k0, wave);
+    cv.pages(a, w, w.k0 + BN, wave);
+    ck.template issue<1>(a, w, w.k0, smem, wave, lane);
+    if (w.k0 + BN < w.k1) cv.template issue<1>(a, w, w.k0 + BN, smem + 2 * TILEB, wave, lane);
+    ck.template issue<2>(a, w, w.k0, smem, wave, lane);
+    ck.pages(a, w, w.k0 + 2 * BN, wave);
+  }
+#pragma unroll
+  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], qrow < w.rows && s * 32 + g16 * 8 < a.hd);
   find_gap(a, lane, w);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(Copy::NI) : "memory");      // both tiles of K
+  if (w.k0 < w.k1) scores(smem, 0);
   int stage = 0;
   for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // the tile is there, and every wave is done with the other one and with the scores
-    if (j0 + BN < w.k1) { cp.issue(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane); cp.pages(a, w, j0 + 2 * BN, wave); }
-    const char* kt = smem + stage * 2 * TILEB;
-    {
-      f32x16_t s, s1;                                          // (two chains: a product that waits for the one before it would idle the unit half of the time)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the scores and V of this tile and K of the next are there, every wave is done with the tile before
+    if (j0 + BN < w.k1) cv.template issue<2>(a, w, j0 + BN, smem + (stage ^ 1) * 2 * TILEB, wave, lane);
+    if (j0 + 2 * BN < w.k1) ck.template issue<1>(a, w, j0 + 2 * BN, smem + stage * 2 * TILEB, wave, lane);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = s1[e] = 0.f;
-#pragma unroll
-      for (int q = 0; q < DS; q += 2) {
-        s = mfma32(*(const bf16x8_t*)(kt + krow + (((kc0 + 2 * q) ^ kswz) << 4)), qf[q], s);
-        s1 = mfma32(*(const bf16x8_t*)(kt + krow + (((kc0 + 2 * q + 2) ^ kswz) << 4)), qf[q + 1], s1);
-      }
-      s += s1;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sx[(wave * 4 + e) * 64 + lane] = (f32x4_t){s[4 * e], s[4 * e + 1], s[4 * e + 2], s[4 * e + 3]};
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int q = 0; q < Copy::PG; ++q) cv.pg[q] = ck.pg[q];
+    ck.pages(a, w, j0 + 3 * BN, wave);
+    if (j0 + BN < w.k1) scores(smem + (stage ^ 1) * 2 * TILEB, stage ^ 1);
     const bool hide = w.gap || j0 + BN - 1 > first, uneven = first < last && j0 + BN - 1 > first;
     uint32_t seen[NB];                                         // bit e: key 8 (e / 4) + 4 half + e % 4
     bf16x8_t pf[NB][2];
@@ -566,11 +592,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
     for (int b = 0; b < NB; ++b) {
       f32x4_t p[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[e] = sx[((b0 + b) * 4 + e) * 64 + lane];
-#pragma unroll
-        for (int q = 1; q < DQ; ++q) p[e] += sx[((2 * q + b0 + b) * 4 + e) * 64 + lane];
-      }
+      for (int e = 0; e < 4; ++e) p[e] = sx[((stage * 2 + (e >> 1)) * 4 + (b0 + b) * 2 + (c32 >> 4)) * 64 + ((e & 1) * 2 + half) * 16 + c16];
       seen[b] = 0xffffu;
       if (hide) {
         seen[b] = 0;
@@ -739,9 +761,12 @@ Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, i
   c.tiles = (long)T * grp / c.bm + R;
   c.cmin = 256;
   const long items = c.tiles * Hkv;
-  // Enough workgroups for two on every CU, down to 256 keys each; and where the keys are many, four times that, so that streams of different lengths even out, but
-  // no fewer than 1024 keys each (a split costs its partial results and the join: with many rows those are as much as the keys, 403 against 440 us without it).
-  const long fill = std::min((2l * cu_count + items - 1) / items, (max_kv + c.cmin - 1) / c.cmin), even = std::min((8l * cu_count + items - 1) / items, c.bm > 16 ? 0l : max_kv / 1024);
+  // Enough workgroups for two on every CU (one and a half, where 128 rows each make a split's partial results dear), down to 256 keys each, or 512 where 64 rows of a
+  // wide head do (chunks of 192 at 800, 4 heads x 512: 71 us whole, 87 in four; 2 x 500 at 1500: 60 in three, 68 in seven); and where rows are few and keys many, four
+  // times that, so that streams of different lengths even out, but no fewer than 1024 keys each (with many rows the partial results and the join are as much
+  // as the keys: 403 against 440 us without it, chunks of 4099 at 4200).
+  const long want = c.bm == 128 ? 3l * cu_count / 2 : 2l * cu_count, most = c.bm == 64 ? max_kv / 512 : (max_kv + c.cmin - 1) / c.cmin;
+  const long fill = std::min((want + items - 1) / items, most), even = c.bm == 16 ? std::min((8l * cu_count + items - 1) / items, max_kv / 1024) : 0;
   c.nsplit = (int)std::max(1l, std::min(std::max(fill, even), (long)MAX_SPLITS));
   return c;
 }
@@ -762,7 +787,7 @@ int launch_tiles(const AttnArgs& a, const Choice& c, hipStream_t st) { return la
 template <int HD>
 int launch_long(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_long_kernel<HD>, 256, 4 * 64 * HD * 2, a, c, st); }
 template <int HD, int NW>
-int launch_wide(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_wide_kernel<HD, NW>, NW * 64, 4 * 32 * HD * 2 + NW * 4096, a, c, st); }
+int launch_wide(const AttnArgs& a, const Choice& c, hipStream_t st) { return launch(paged_attn_wide_kernel<HD, NW>, NW * 64, 4 * 32 * HD * 2 + 2 * 8192, a, c, st); }
 constexpr int CUS = 256;
 }  // namespace
 
