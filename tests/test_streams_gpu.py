@@ -435,7 +435,8 @@ def w4_in_64(x, w, bias, act, res):
 
 
 @pytest.mark.parametrize('M,N,K,group', [(1, 2048, 2048, 128), (3, 100, 8192, 64), (1, 1, 32, 32), (2, 17, 96, 32), (16, 64, 192, 64), (17, 33, 256, 128), (5, 427, 1408, 128),
-                                         (33, 1000, 512, 32), (64, 48, 1024, 64), (65, 50, 384, 128), (200, 130, 640, 32), (7, 15, 8192, 128), (4, 96, 11008, 64)])
+                                         (33, 1000, 512, 32), (64, 48, 1024, 64), (65, 50, 384, 128), (200, 130, 640, 32), (7, 15, 8192, 128), (4, 96, 10944, 64),
+                                         (20, 12300, 256, 64), (21, 70, 384, 128), (36, 12300, 256, 128), (37, 6200, 160, 32), (48, 6200, 256, 128)])
 @pytest.mark.parametrize('epi', ['plain', 'bias', 'gelu', 'res', 'all', 'f32'])
 def test_w4_linear_against_64_bits(ops, M, N, K, group, epi):
     g = torch.Generator(device='cuda').manual_seed(M * 1000 + N + K)
