@@ -28,6 +28,7 @@ struct AttnArgs {
   long ldq, ldo, npages;
   int shift, ldt, width, T, R, H, Hkv, grp, hd, nsplit, cmin;
   float scale_log2;                                            // |scale| log2(e): exponentials are powers of two
+  uint32_t rowe;                                               // elements of a token's row in a cache: Hkv hd
   uint32_t q_and, q_xor;                                       // applied to q as it is read: the sign of a negative scale; a scale of 0 is a q of 0
 };
 
@@ -76,6 +77,7 @@ struct Work {
   bool gap;                                                    // some table entry of the range names no page
   int entry;                                                   // this lane's entry of the range (its first 64)
   table_t tab;
+  const bf16_t *kc, *vc;                                       // the kv head's columns of the caches
 };
 __device__ __forceinline__ int row_pos(const Work& w, int row, int grp) { return w.kv - w.n + row / grp; }
 // (All 64 lanes probe at once, and the last probe brings the stream's numbers with it: what a workgroup waits for before its first copy is this, the page and no more.)
@@ -108,6 +110,8 @@ __device__ __forceinline__ bool find_work(const AttnArgs& a, int bm, int lane, W
   w.k1 = (int)min((long)(w.sp + 1) * chunk, (long)(last + 1));
   if (w.k0 >= w.k1 && a.nsplit > 1) return false;              // (the join knows)
   w.tab = (table_t)(a.table + (size_t)r * a.ldt);
+  w.kc = a.kc + (size_t)w.hk * a.hd;
+  w.vc = a.vc + (size_t)w.hk * a.hd;
   w.gap = true;                                                // until find_gap, which nothing waits for before the first copies are out
   w.entry = w.tab[max(0, min((w.k0 >> a.shift) + lane, (w.k1 - 1) >> a.shift))];
   return true;
@@ -132,7 +136,7 @@ struct Copier {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int at = i * 1024 + lane * 16, row = at / ROWB, c = ((at % ROWB) >> 4) ^ SWZ(wave * RW + row);
-      off[i] = c * 8 < a.hd ? (uint32_t)(((row % RP) * a.Hkv * a.hd + c * 8) * 2) : NONE;
+      off[i] = c * 8 < a.hd ? (uint32_t)(((row % RP) * a.rowe + c * 8) * 2) : NONE;
     }
   }
   __device__ __forceinline__ void pages(const AttnArgs& a, const Work& w, int j0, int wave) {      // of the tile that is issued next
@@ -142,18 +146,22 @@ struct Copier {
   // K: to dst, V: to dst + TILEB; WHICH: 1 K, 2 V, 3 both
   template <int WHICH>
   __device__ __forceinline__ void issue(const AttnArgs& a, const Work& w, int j0, char* dst, int wave, int lane) {
-    const bool whole = j0 + BN <= w.k1 && !w.gap;
+    if (j0 + BN <= w.k1 && !w.gap) put<WHICH, true>(a, w, j0, dst, wave, lane);
+    else put<WHICH, false>(a, w, j0, dst, wave, lane);
+  }
+  template <int WHICH, bool WHOLE>
+  __device__ __forceinline__ void put(const AttnArgs& a, const Work& w, int j0, char* dst, int wave, int lane) {
 #pragma unroll
     for (int q = 0; q < PG; ++q) {
       const int jb = j0 + wave * RW + q * RP;
-      const size_t at = ((((size_t)(uint32_t)pg[q] << a.shift) + (jb & ((1 << a.shift) - 1))) * a.Hkv + w.hk) * a.hd;
-      const bool there = pg[q] >= 0 && pg[q] < a.npages;
+      const size_t at = (((size_t)(uint32_t)pg[q] << a.shift) + (jb & ((1 << a.shift) - 1))) * a.rowe;
+      const bool there = WHOLE || (pg[q] >= 0 && pg[q] < a.npages);
 #pragma unroll
       for (int i = q * NI / PG; i < (q + 1) * NI / PG; ++i) {
         uint32_t v = off[i];
-        if (!whole && (jb + (i * 1024 + lane * 16) / ROWB % RP >= w.k1 || !there)) v = NONE;
-        if constexpr (WHICH & 1) copy(a.kc + at, dst + wave * (TILEB / NW) + i * 1024, v);
-        if constexpr (WHICH & 2) copy(a.vc + at, dst + TILEB + wave * (TILEB / NW) + i * 1024, v);
+        if constexpr (!WHOLE) { if (jb + (i * 1024 + lane * 16) / ROWB % RP >= w.k1 || !there) v = NONE; }
+        if constexpr (WHICH & 1) copy(w.kc + at, dst + wave * (TILEB / NW) + i * 1024, v);
+        if constexpr (WHICH & 2) copy(w.vc + at, dst + TILEB + wave * (TILEB / NW) + i * 1024, v);
       }
     }
   }
@@ -357,6 +365,10 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
 // row's maximum and sum are 31 operations and one exchange of the wave's halves), P^T is already the right operand of O^T = V^T P^T.  No wave waits for another but
 // for the tile.  The running maximum follows only when a score passes it by more than 2^8: the probabilities then stay below 2^8, where bf16 and the fp32
 // sums are as exact as below 1, and the accumulators are rarely rescaled.
+//   Two workgroups share a CU, two waves a SIMD, of which one's softmax is to run beside the other's products: chunks of 4099 at 4200, 16 / 4 heads x 128, take
+// 365 to 376 us, 0.85 PFLOP/s.  What that cost to reach: half of the score operands read ahead of their products, the products' waves given precedence and V's next
+// fragments read ahead (437 -> 414 us); a copy of a whole tile in a path of its own, so that it is eight instructions and their addresses (404 -> 374); a row's
+// visible keys in bits of a register, not in 64 scalar registers that pushed the loop's own ones out (4 x 1000 at 1000, 12 heads x 64: 59 -> 54).
 template <int HD>
 __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
   constexpr int BN = 64, BM = 128, ROWB = HD * 2, TILEB = BN * ROWB, DS = HD / 16, DT = HD / 32;
@@ -405,12 +417,24 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
     f32x16_t s[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int q = 0; q < DS; ++q)
+    for (int q0 = 0; q0 < DS; q0 += 4) {
+      bf16x8_t kf[4][2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) s[k] = mfma32(*(const bf16x8_t*)(kt + k * 32 * ROWB + krow + (((2 * q + half) ^ kswz) << 4)), qf[q], s[k]);
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) kf[q][k] = *(const bf16x8_t*)(kt + k * 32 * ROWB + krow + (((2 * (q0 + q) + half) ^ kswz) << 4));
+      __builtin_amdgcn_sched_barrier(0);                       // (left alone, the compiler reads two fragments ahead of the products and waits for each)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) s[k] = mfma32(kf[q][k], qf[q0 + q], s[k]);
+    }
+    __builtin_amdgcn_s_setprio(0);
     uint32_t seen = 0xffffffffu;                               // bit 16 k + e: key 32 k + 8 (e / 4) + 4 half + e % 4
     if (w.gap || j0 + BN - 1 > first) {
+      const int lim = min(pos, w.k1 - 1);
       seen = 0;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
@@ -419,11 +443,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
           const int j = j0 + k * 32 + e4 * 8 + half * 4;
           const bool there = page_there(a, w, j);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool see = there && j + e <= pos && j + e < w.k1;
-            s[k][e4 * 4 + e] = see ? s[k][e4 * 4 + e] : -INFINITY;
-            seen |= (uint32_t)see << (k * 16 + e4 * 4 + e);
-          }
+          for (int e = 0; e < 4; ++e) seen |= (uint32_t)(there && j + e <= lim) << (k * 16 + e4 * 4 + e);
+          asm volatile("" : "+v"(seen));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[k][e4 * 4 + e] = (seen >> (k * 16 + e4 * 4 + e)) & 1u ? s[k][e4 * 4 + e] : -INFINITY;
         }
     }
     float mx = -INFINITY;
@@ -450,18 +473,29 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
         pf[2 * k + t] = __builtin_bit_cast(bf16x8_t, (u32x4_t){pack2bf(s[k][8 * t], s[k][8 * t + 1]), pack2bf(s[k][8 * t + 2], s[k][8 * t + 3]),
                                                                pack2bf(s[k][8 * t + 4], s[k][8 * t + 5]), pack2bf(s[k][8 * t + 6], s[k][8 * t + 7])});
     }
+    __builtin_amdgcn_s_setprio(1);
     const uint32_t va = vaddr0 + stage * 2 * TILEB, vb = va ^ 32;       // rows + 8: the swizzle differs by two pieces
     // (a tile of which one row sees a key that another one does not: a value that is not finite must not reach the latter through its probability of 0)
     const bool uneven = first < last && j0 + BN - 1 > first;
+    bf16x8_t vbuf[2][4];                                       // (the fragments of the next columns are read while these are multiplied)
+    const auto read_v = [&](int d) {
+      const uint32_t x = va ^ (d * 64), y = vb ^ (d * 64);
+      bf16x8_t* v = vbuf[d & 1];
+      v[0] = tr_join(ds_read_tr_na<0>(x), ds_read_tr_na<8 * ROWB>(y));
+      v[1] = tr_join(ds_read_tr_na<16 * ROWB>(x), ds_read_tr_na<24 * ROWB>(y));
+      v[2] = tr_join(ds_read_tr_na<32 * ROWB>(x), ds_read_tr_na<40 * ROWB>(y));
+      v[3] = tr_join(ds_read_tr_na<48 * ROWB>(x), ds_read_tr_na<56 * ROWB>(y));
+    };
+    read_v(0);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      bf16x8_t vf[4];
-      const uint32_t x = va ^ (d * 64), y = vb ^ (d * 64);
-      vf[0] = tr_join(ds_read_tr_na<0>(x), ds_read_tr_na<8 * ROWB>(y));
-      vf[1] = tr_join(ds_read_tr_na<16 * ROWB>(x), ds_read_tr_na<24 * ROWB>(y));
-      vf[2] = tr_join(ds_read_tr_na<32 * ROWB>(x), ds_read_tr_na<40 * ROWB>(y));
-      vf[3] = tr_join(ds_read_tr_na<48 * ROWB>(x), ds_read_tr_na<56 * ROWB>(y));
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vf[0]), "+v"(vf[1]), "+v"(vf[2]), "+v"(vf[3])::"memory");
+      bf16x8_t* vf = vbuf[d & 1];
+      if (d + 1 < DT) {
+        read_v(d + 1);
+        asm volatile("s_waitcnt lgkmcnt(8)" : "+v"(vf[0]), "+v"(vf[1]), "+v"(vf[2]), "+v"(vf[3])::"memory");
+      } else {
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vf[0]), "+v"(vf[1]), "+v"(vf[2]), "+v"(vf[3])::"memory");
+      }
       if (uneven) {
         if (__any(not_finite(vf[0]) || not_finite(vf[1]) || not_finite(vf[2]) || not_finite(vf[3]))) {
           f32x16_t c;
@@ -480,6 +514,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) o[d] = mfma32(vf[t], pf[t], o[d]);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
   l += __shfl_xor(l, 32, 64);
   if (!ok) return;
@@ -595,17 +630,17 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
       for (int e = 0; e < 4; ++e) p[e] = sx[((stage * 2 + (e >> 1)) * 4 + (b0 + b) * 2 + (c32 >> 4)) * 64 + ((e & 1) * 2 + half) * 16 + c16];
       seen[b] = 0xffffu;
       if (hide) {
+        const int lim = min(pos[b], w.k1 - 1);
         seen[b] = 0;
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4) {
           const int j = j0 + e4 * 8 + half * 4;
           const bool there = page_there(a, w, j);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool see = there && j + e <= pos[b] && j + e < w.k1;
-            p[e4][e] = see ? p[e4][e] : -INFINITY;
-            seen[b] |= (uint32_t)see << (e4 * 4 + e);
-          }
+          for (int e = 0; e < 4; ++e) seen[b] |= (uint32_t)(there && j + e <= lim) << (e4 * 4 + e);
+          asm volatile("" : "+v"(seen[b]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[e4][e] = (seen[b] >> (e4 * 4 + e)) & 1u ? p[e4][e] : -INFINITY;
         }
       }
       float mx = -INFINITY;
@@ -802,7 +837,7 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   AVT_CHECK(T >= 0 && R >= 1 && H >= 1 && Hkv >= 1 && H % Hkv == 0, "avt_paged_attn_fwd: bad sizes (T %d, R %d, H %d, Hkv %d)", T, R, H, Hkv);
   AVT_CHECK(head_dim >= 8 && head_dim % 8 == 0 && head_dim <= HDMAX, "avt_paged_attn_fwd: head_dim must be a multiple of 8 in [8, %d] (got %d)", HDMAX, head_dim);
   AVT_CHECK(page >= 8 && page <= 1024 && (page & (page - 1)) == 0, "avt_paged_attn_fwd: the page must be a power of two in [8, 1024] (got %d)", page);
-  AVT_CHECK(npages >= 0 && width >= 1 && ldt >= width && (long)width * page <= 0x7fffffffl, "avt_paged_attn_fwd: bad table (width %d, ldt %d, page %d)", width, ldt, page);
+  AVT_CHECK(npages >= 0 && width >= 1 && ldt >= width && (long)width * page < 0x7fff0000l, "avt_paged_attn_fwd: bad table (width %d, ldt %d, page %d)", width, ldt, page);
   if (T == 0) return 0;
   AVT_CHECK(q && kcache && vcache && table && cu && kv_lens && out, "avt_paged_attn_fwd: null argument");
   AVT_CHECK(ldq >= (long)H * head_dim && ldo >= (long)H * head_dim && ldq % 8 == 0 && ldo % 8 == 0 && aligned16(q) && aligned16(kcache) && aligned16(vcache) && aligned16(out),
@@ -818,6 +853,7 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   a.part_o = (float*)ws; a.part_ml = (float*)ws + (size_t)c.nsplit * T * H * head_dim;
   a.ldq = ldq; a.ldo = ldo; a.npages = npages; a.shift = __builtin_ctz(page); a.ldt = ldt; a.width = width; a.T = T; a.R = R; a.H = H; a.Hkv = Hkv; a.grp = H / Hkv;
   a.hd = head_dim; a.nsplit = c.nsplit; a.cmin = c.cmin; a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
+  a.rowe = (uint32_t)Hkv * head_dim;
   a.q_and = scale == 0.f ? 0u : 0xffffffffu; a.q_xor = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t st = (hipStream_t)stream;
   int rc = 0;
