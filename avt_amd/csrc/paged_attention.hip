@@ -550,12 +550,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
 #pragma unroll
   for (int b = 0; b < NB; ++b) { const int row = w.row0 + (b0 + b) * 32 + c32; pos[b] = row < w.rows ? row_pos(w, row, a.grp) : -1; }
   bf16x8_t qf[DS];
-  const int qrow = w.row0 + rb * 16 + c16;
+  // (which columns a product of the scores takes is free, so lane group g has those of quarter g: whichever lanes the LDS serves together, their 16 rows then lie on
+  // 16 different slots.  With 32 neighbouring columns to a product a third of the LDS cycles were conflicts.)
+  const int qrow = w.row0 + rb * 16 + c16, qcol = g16 * (HD / 4);
   {
     const int row = min(qrow, w.rows - 1), tok = row / a.grp;
     const bf16_t* p = a.q + (size_t)(w.t0 + tok) * a.ldq + (size_t)(w.hk * a.grp + row - tok * a.grp) * a.hd;
 #pragma unroll
-    for (int s = 0; s < DS; ++s) qf[s] = *(const bf16x8_t*)(p + (s * 32 + g16 * 8 < a.hd ? s * 32 + g16 * 8 : 0));
+    for (int s = 0; s < DS; ++s) qf[s] = *(const bf16x8_t*)(p + (qcol + s * 8 < a.hd ? qcol + s * 8 : 0));
   }
   f32x16_t o[NB][DT];
   float m[NB], l[NB];
@@ -581,7 +583,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
       for (int q0 = 0; q0 < DS; q0 += 8) {
         bf16x8_t kf[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) kf[q] = *(const bf16x8_t*)(kr + (((4 * (q0 + q) + g16) ^ kswz) << 4));
+        for (int q = 0; q < 8; ++q) kf[q] = *(const bf16x8_t*)(kr + (((g16 * (HD / 32) + q0 + q) ^ kswz) << 4));
         __builtin_amdgcn_sched_barrier(0);                     // (left alone, the compiler reads two fragments ahead of the products and waits for each)
 #pragma unroll
         for (int q = 0; q < 8; q += 2) {
@@ -607,7 +609,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
     ck.pages(a, w, w.k0 + 2 * BN, wave);
   }
 #pragma unroll
-  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], qrow < w.rows && s * 32 + g16 * 8 < a.hd);
+  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], qrow < w.rows && qcol + s * 8 < a.hd);
   find_gap(a, lane, w);
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(Copy::NI) : "memory");      // both tiles of K
   if (w.k0 < w.k1) scores(smem, 0);
