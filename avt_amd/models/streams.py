@@ -161,7 +161,10 @@ class HeadStreams:
 
     def release(self, which):
         """Streams ``which`` give their pages back and are empty."""
-        for s in {int(s) for s in which}:
+        which = {int(s) for s in which}
+        if any(not 0 <= s < self.S for s in which):
+            raise ValueError(f'release: streams 0 to {self.S - 1}, got {sorted(which)}')
+        for s in which:
             n = self._owned[s]
             self.free[self._n_free:self._n_free + n].copy_(self.table[s, :n])
             self._n_free += n

@@ -328,7 +328,7 @@ int avt_sgd_step_dev(float* param, float* grad, float* momentum_buf, void* shado
 /* ---- many streams on one paged key / value cache (ABI 10) ---------------------------------------------------------------
  * What `past_key_values` is to one batch of clips of one length (models/future_prediction.py:168-202), for streams of different lengths that grow by
  * chunks: a pool of pages of `page` tokens (a power of two in [8, 1024]), kcache / vcache bf16 [npages][page][Hkv][head_dim], and per stream a row of
- * `width` page numbers in `table` (int32, row stride ldt).  All int32 arrays live on the device, so a step can be captured and replayed.
+ * `width` page numbers in `table` (int32, row stride ldt; width * page < 2^31 - 2^16).  All int32 arrays live on the device, so a step can be captured and replayed.
  * avt_paged_plan: R <= 4096 streams of lens[r] cached tokens that own owned[r] pages each take fresh[r] >= 0 new tokens, packed one stream behind the
  *   other into T token rows; free_pages[0 .. *n_free) (at most nfree_max) is a stack of free pages.
  *     cu [R + 1]      first token row of each stream (running sum of fresh);  rows behind cu[R]: slot, position and stream -1
@@ -345,7 +345,10 @@ int avt_sgd_step_dev(float* param, float* grad, float* momentum_buf, void* shado
  *   Rows behind cu[R] are left as they are.  head_dim % 8 == 0, <= 1024.  max_new / max_kv: what the caller knows of the longest chunk and of the longest
  *   kv_lens (0: nothing); they choose kernels and grids, results hold for any lengths.  ws: avt_paged_attn_workspace_bytes of the same arguments.
  * avt_w4_linear: y[m, n] = epilogue(sum_k x[m, k] s[n, k / group] (u[n, k] - 8)): x bf16 [M][K], u in 0 .. 15 two to a byte (q [N][K / 2], the low nibble holds
- *   the even k), s bf16 [N][K / group], group 32 / 64 / 128; + bias (fp32), act 2: tanh GELU, + res (bf16); out_mode 0: bf16, 1: fp32. */
+ *   the even k), s bf16 [N][K / group], group 32 / 64 / 128; + bias (fp32), act 2: tanh GELU, + res (bf16); out_mode 0: bf16, 1: fp32.
+ *   The weights are never rounded: 16 + u is exact in bf16, and 24 times the group's sum of x is taken off in fp32, so sums of 31 |x| have to stay in fp32's
+ *   range; a row of x that is not finite gives NaN or infinities in its own outputs and in no others.  No output may overlap an input, here and above, but
+ *   out == res of the same strides. */
 int avt_paged_plan(const int* lens, const int* fresh, const int* owned, int* table, int ldt, int width, const int* free_pages, int nfree_max,
                    const int* n_free, int page, int R, int T, int* cu, int* kv_lens, int* owned_out, int* n_free_out, int* slots, int* positions,
                    int* streams, void* stream);

@@ -584,6 +584,21 @@ def test_streams_release_and_refuse(ops):
             head.open_streams(2, **kw)
 
 
+def test_streams_release_of_what_is_not_there(ops):
+    """Refused as a whole: a number that is no stream (a negative one would count from the end) leaves every stream and page where it was."""
+    head, orc = build_head(64, 64, 2, 2)
+    st = head.open_streams(2, max_len=40, page=8, pages=7)
+    x = torch.randn((20, 64), generator=torch.Generator().manual_seed(3))
+    st.append(x[:15].cuda(), [9, 6])
+    for which in ([0, 2], [-1], [1, 99]):
+        with pytest.raises(ValueError, match='release'):
+            st.release(which)
+    assert st.lengths == [9, 6] and int(st.n_free) == 4
+    out = st.append(x[15:17].cuda(), [1, 1])
+    close(out[:1], oracle_decode(orc, torch.cat([x[:9], x[15:16]]), 1)[9:])
+    close(out[1:], oracle_decode(orc, torch.cat([x[9:15], x[16:17]]), 1)[6:])
+
+
 def test_streams_on_four_bit_weights(ops):
     """The same as a head whose projections hold the values that the 4-bit weights stand for."""
     head, _ = build_head(128, 256, 3, 2)
