@@ -38,8 +38,10 @@ __device__ __forceinline__ void copy_to_lds(const void* base, char* lds, uint32_
 }
 
 // One workgroup (8 waves) per NT * 16 columns and up to MT * 16 rows; the waves take steps of 128 k in turn, and their sums meet in LDS, added in the order of
-// the waves.  Products are of the exact integers 16 + u with the bf16 x, in fp32, and a group ends with y += s (sum - 24 sum x): the weights are never rounded.
-// sum x comes from a product with ones, in the same layout.
+// the waves.  Products are of the exact integers 16 + u with the bf16 x, in fp32, and begin at -24 sum x, a product with a matrix of -24, so a group ends with
+// y += s sum: the weights are never rounded.
+//   1 x 2048 x 2048 3.3 us, 3 x 2048 x 8192 7.8 us, both the launch and one round of loads; 1 x 16384 x 8192 16.1 us, 4.3 TB/s of weights and scales; 33 rows of
+// the same 27.5 us: 18.8 without the products, whose operands (weights unpacked, x paired, a wave's 3 x 4 tiles in 250 registers) leave two waves a SIMD.
 //   A load whose neighbouring lanes read different rows takes the vector cache 4 cycles per 64 bytes (measured: 59 cycles for 64 x 16 bytes of 16 rows, and these
 // loads, not the bytes, set the time: 43 us of 33 x 16384 x 8192 against 24 without those of x), but that is how the matrix unit wants its operands.  So neighbouring
 // lanes fetch neighbouring bytes -- weights 64 bytes of each of 16 rows, copied straight into LDS, x 256 bytes of each of 4 rows, through registers -- and a wave
@@ -57,7 +59,7 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4Args a) {
   char* xl = wl + 2 * NT * 1024;
   const size_t rowb = (size_t)a.K / 2;
   const int full = a.K / 128;
-  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  const bf16x8_t minus24 = __builtin_bit_cast(bf16x8_t, (u32x4_t){0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u});
   // (addresses: a uniform base, which moves with the step, and 32-bit lane offsets)
   const uint8_t* qb = a.q + (size_t)n0 * rowb;
   const bf16_t* sb = a.s + (size_t)n0 * a.groups;
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4Args a) {
 #pragma unroll
         for (int q = 0; q < GS; ++q) {
           xf[i][e * GS + q] = pair8(__builtin_bit_cast(u32x4_t, xf[i][e * GS + q]));
-          xs[i] = mfma16(xf[i][e * GS + q], ones, xs[i]);
+          xs[i] = mfma16(xf[i][e * GS + q], minus24, xs[i]);
         }
       }
 #pragma unroll
@@ -138,15 +140,16 @@ __global__ __launch_bounds__(512) void w4_linear_kernel(W4Args a) {
         bf16x8_t wf[GS];
 #pragma unroll
         for (int q = 0; q < GS; ++q) wf[q] = unpack8(w[j][e * GS + q]);
+        f32x4_t acc[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < GS; ++q)
 #pragma unroll
-          for (int q = 0; q < GS; ++q) acc = mfma16(xf[i][e * GS + q], wf[q], acc);
-          const float s = __uint_as_float(sc[j * GPS + e] << 16);
+          for (int i = 0; i < MT; ++i) acc[i] = mfma16(xf[i][e * GS + q], wf[q], q ? acc[i] : xs[i]);
+        const float s = __uint_as_float(sc[j * GPS + e] << 16);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[j][i][r] = fmaf(s, fmaf(-24.f, xs[i][r], acc[r]), y[j][i][r]);
-        }
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[j][i][r] = fmaf(s, acc[i][r], y[j][i][r]);
       }
     }
   };
