@@ -796,14 +796,19 @@ Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, i
   const long rows = (max_new > 0 && max_new < T ? max_new : (T + R - 1) / R) * grp;      // rows of a stream and kv head
   c.bm = rows <= 16 || c.hd == 1024 ? 16 : c.hd <= 128 ? 128 : 64;
   c.tiles = (long)T * grp / c.bm + R;
-  c.cmin = 256;
+  c.cmin = c.bm == 16 ? 64 : 256;
   const long items = c.tiles * Hkv;
-  // Enough workgroups for two on every CU (one and a half, where 128 rows each make a split's partial results dear), down to 256 keys each, or 512 where 64 rows of a
-  // wide head do (chunks of 192 at 800, 4 heads x 512: 71 us whole, 87 in four; 2 x 500 at 1500: 60 in three, 68 in seven); and where rows are few and keys many, four
-  // times that, so that streams of different lengths even out, but no fewer than 1024 keys each (with many rows the partial results and the join are as much
-  // as the keys: 403 against 440 us without it, chunks of 4099 at 4200).
-  const long want = c.bm == 128 ? 3l * cu_count / 2 : 2l * cu_count, most = c.bm == 64 ? max_kv / 512 : (max_kv + c.cmin - 1) / c.cmin;
-  const long fill = std::min((want + items - 1) / items, most), even = c.bm == 16 ? std::min((8l * cu_count + items - 1) / items, max_kv / 1024) : 0;
+  // Enough workgroups for two on every CU (one and a half, where 128 rows each make a split's partial results dear), down to 64 keys each of few rows (a tile of 16
+  // to 64 keys is 0.9 us of latency, a join 4: 1 x 730, 8 heads x 128, 14 us in splits of 256 keys, 9.4 in splits of 64), 256 of 128 rows and 512 of 64 rows of a
+  // wide head (chunks of 192 at 800, 4 heads x 512: 71 us whole, 87 in four).  With many rows, only to have one on every CU, down to 128 keys (3 x 680 at 1168, one
+  // head x 128: 24 us in 8, 21 in 15; 32 x 40 at 500, 8 / 2 heads x 128, which has enough: 21 us in splits of 256 keys, 25 in splits of 128).
+  // And where rows are few and keys many, four times that, so that streams of different lengths even out, but no fewer than 1024 keys each (with many rows the
+  // partial results and the join are as much as the keys: 403 against 440 us without it, chunks of 4099 at 4200).
+  const long want = c.bm == 128 ? 3l * cu_count / 2 : 2l * cu_count;
+  const long most = c.bm == 64 ? max_kv / 512 : (max_kv + c.cmin - 1) / c.cmin, one = max_kv < 192 ? 1 : std::min(cu_count / items, (max_kv + 127) / 128);
+  long fill = std::min((want + items - 1) / items, most);
+  if (c.bm > 16 && one > fill) { fill = one; c.cmin = 128; }
+  const long even = c.bm == 16 ? std::min((8l * cu_count + items - 1) / items, max_kv / 1024) : 0;
   c.nsplit = (int)std::max(1l, std::min(std::max(fill, even), (long)MAX_SPLITS));
   return c;
 }
