@@ -171,6 +171,22 @@ struct Copier {
   }
 };
 
+// The 64 rows of Q of a workgroup, where the first two tiles of V will be (rows 0 .. 31 in the first one's place): whole rows, neighbouring lanes on neighbouring
+// bytes (fetched as a product wants them, 64 lanes on 16 or more rows: 11 x 976 at 42, 8 / 2 heads x 512, 180 us, now 170).  Rows and columns that are not there are zeros.
+template <int HD, int NW>
+__device__ __forceinline__ void copy_q(const AttnArgs& a, const Work& w, char* smem, int wave, int lane) {
+  constexpr int ROWB = HD * 2, TILEB = 32 * ROWB, RPI = 1024 / ROWB, NI = 64 / RPI / NW;      // rows of an instruction, instructions of a wave
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = (wave * NI + i) * RPI, row = min(w.row0 + r, w.rows - 1), tok = row / a.grp, h = row - tok * a.grp;
+    const bf16_t* base = a.q + (size_t)(w.t0 + tok) * a.ldq + (size_t)(w.hk * a.grp + h) * a.hd;
+    const int sub = lane * 16 / ROWB, c = (lane * 16 % ROWB >> 4) ^ swz32<HD>((r + sub) & 31);
+    const uint32_t next = (uint32_t)(h + 1 < a.grp ? a.hd : a.ldq - (long)(a.grp - 1) * a.hd);      // from a row to the one behind it
+    Copier<HD, 32, NW, swz32<HD>>::copy(base, smem + (r < 32 ? TILEB : 3 * TILEB) + (r & 31) * ROWB,
+                                        w.row0 + r + sub < w.rows && c * 8 < a.hd ? (sub * next + c * 8) * 2 : 0xFFFFFFF0u);
+  }
+}
+
 // A V fragment of a tile that some row sees a part of: values that are not finite are taken out (their rows' probabilities may be 0) and told from `code`, which is
 // 1 for a NaN, 2^8 for +inf and 2^16 for -inf: its product with the rows' visibility counts, exactly, what each row sees of them.
 __device__ __forceinline__ bool not_finite(bf16x8_t f) {
@@ -535,6 +551,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
 // the 256 registers that the vector unit reaches (with 4 waves for 512 columns the compiler kept O in the others and moved it to and fro: 8 us a tile).
 // The scores of tile i + 1 are made between the same two barriers as the softmax and the products with V of tile i, so that neither unit waits for the other.
 // Maximum and sum of a row are kept by every wave that has a part of it, as in the kernel for few rows, and follow as in the one for many.
+//   Chunks of 192 at 800, 4 heads x 512, take 65 us, 180 TFLOP/s: neither the bytes (44 us with the copies alone) nor the products (14 % of the matrix unit's cycles)
+// but a wave's own chain through a tile, 430 instructions and four trips to LDS of which the other wave of its SIMD hides a part, and workgroups that fill a CU alone.
 template <int HD, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a) {
   constexpr int BN = 32, BM = 64, ROWB = HD * 2, TILEB = BN * ROWB, DS = HD / 32, KB = 8 / NW, DT = HD / 128, NB = 8 / NW;      // KB: key blocks of a wave's S, NB: row blocks of its O
@@ -550,15 +568,6 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
 #pragma unroll
   for (int b = 0; b < NB; ++b) { const int row = w.row0 + (b0 + b) * 32 + c32; pos[b] = row < w.rows ? row_pos(w, row, a.grp) : -1; }
   bf16x8_t qf[DS];
-  // (which columns a product of the scores takes is free, so lane group g has those of quarter g: whichever lanes the LDS serves together, their 16 rows then lie on
-  // 16 different slots.  With 32 neighbouring columns to a product a third of the LDS cycles were conflicts.)
-  const int qrow = w.row0 + rb * 16 + c16, qcol = g16 * (HD / 4);
-  {
-    const int row = min(qrow, w.rows - 1), tok = row / a.grp;
-    const bf16_t* p = a.q + (size_t)(w.t0 + tok) * a.ldq + (size_t)(w.hk * a.grp + row - tok * a.grp) * a.hd;
-#pragma unroll
-    for (int s = 0; s < DS; ++s) qf[s] = *(const bf16x8_t*)(p + (qcol + s * 8 < a.hd ? qcol + s * 8 : 0));
-  }
   f32x16_t o[NB][DT];
   float m[NB], l[NB];
 #pragma unroll
@@ -605,14 +614,25 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
     cv.pages(a, w, w.k0 + BN, wave);
     ck.template issue<1>(a, w, w.k0, smem, wave, lane);
     if (w.k0 + BN < w.k1) cv.template issue<1>(a, w, w.k0 + BN, smem + 2 * TILEB, wave, lane);
+    copy_q<HD, NW>(a, w, smem, wave, lane);
+  }
+  find_gap(a, lane, w);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");       // Q and both tiles of K
+  {
+    const char* qr = smem + (rb < 2 ? TILEB : 3 * TILEB) + ((rb & 1) * 16 + c16) * ROWB;
+    const int qswz = swz32<HD>((rb & 1) * 16 + c16);
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      qf[s] = *(const bf16x8_t*)(qr + (((g16 * (HD / 32) + s) ^ qswz) << 4));
+      prepare_q(a, qf[s], true);
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wave has its part of Q: V may take its place
+  if (w.k0 < w.k1) {
     ck.template issue<2>(a, w, w.k0, smem, wave, lane);
     ck.pages(a, w, w.k0 + 2 * BN, wave);
+    scores(smem, 0);
   }
-#pragma unroll
-  for (int s = 0; s < DS; ++s) prepare_q(a, qf[s], qrow < w.rows && qcol + s * 8 < a.hd);
-  find_gap(a, lane, w);
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(Copy::NI) : "memory");      // both tiles of K
-  if (w.k0 < w.k1) scores(smem, 0);
   int stage = 0;
   for (int j0 = w.k0; j0 < w.k1; j0 += BN, stage ^= 1) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // the scores and V of this tile and K of the next are there, every wave is done with the tile before
@@ -849,6 +869,7 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   AVT_CHECK(q && kcache && vcache && table && cu && kv_lens && out, "avt_paged_attn_fwd: null argument");
   AVT_CHECK(ldq >= (long)H * head_dim && ldo >= (long)H * head_dim && ldq % 8 == 0 && ldo % 8 == 0 && aligned16(q) && aligned16(kcache) && aligned16(vcache) && aligned16(out),
             "avt_paged_attn_fwd: 16-byte aligned rows required");
+  AVT_CHECK(ldq < (1l << 29), "avt_paged_attn_fwd: rows of q are too far apart (%ld)", ldq);
   AVT_CHECK((long)Hkv * head_dim < (1l << 26), "avt_paged_attn_fwd: a token's row is too long (%d heads of %d)", Hkv, head_dim);
   AVT_CHECK((long)T * H < 0x7f000000l, "avt_paged_attn_fwd: too many rows for one call (%d tokens of %d heads)", T, H);
   const Choice c = choose(T, R, H, Hkv, head_dim, max_new, max_kv > 0 ? max_kv : 0x7fffffff, CUS);
