@@ -240,6 +240,8 @@ __device__ __forceinline__ bool page_there(const AttnArgs& a, const Work& w, int
 // columns (w / KT); the scores pass through LDS (16 bytes per lane, the same lane reads them) and every wave then has all of them in the layout of P^T, the right
 // operand of O^T = V^T P^T, and keeps the running maximum and sum (fp32) of every row for itself: no reduction between waves.  Wave w owns a quarter of the head's
 // columns of O.  P is rounded to bf16 for the product (the matrix unit's type; half a step 2^-8 of each probability), the sum is of the unrounded ones.
+//   Bound by the cache's bytes where there are many streams: 60 x 1 at 9000, 32 / 8 heads x 128, 265 us and 7 of the join, 4.9 TB/s, a large copy's rate; 64 x 1 at
+// 1023, 4 heads x 512, 66 us and 4.  Of few short streams, by the chain cu, table, page, key, score, value: 5.6 us for 3 x 1 at 14.
 template <int HD, int BN>
 __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
   constexpr int ROWB = HD * 2, TILEB = BN * ROWB, KT = BN / 16, KS = 4 / KT, DS = HD / KS / 32, DT = HD / 64, TT = BN >= 32 ? BN / 32 : 1, BM = 16;
@@ -751,7 +753,8 @@ __device__ __forceinline__ int splits_of(const AttnArgs& a, int t, int lane) {
   const int pos = kv - n + (t - t0);
   return pos < 0 ? 0 : (int)(pos / split_keys(kv, a.nsplit, a.cmin)) + 1;
 }
-// Few splits (up to FEW_SPLITS; many rows): a thread takes four columns of a row through all of them.
+// Few splits (up to FEW_SPLITS; many rows): a thread takes four columns of a row through all of them.  Bound by the partial results' bytes, 8 a column, row and split:
+// 8 x 300 at 2000, 8 heads x 256 in two, 10.4 us; 4 us at the least, a launch and two dependent loads.
 __global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
   const int t = blockIdx.x, nz = splits_of(a, t, threadIdx.x & 63);
   const int idx = blockIdx.y * 256 + threadIdx.x;
