@@ -384,7 +384,7 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
 // for the tile.  The running maximum follows only when a score passes it by more than 2^8: the probabilities then stay below 2^8, where bf16 and the fp32
 // sums are as exact as below 1, and the accumulators are rarely rescaled.
 //   Two workgroups share a CU, two waves a SIMD, of which one's softmax is to run beside the other's products: chunks of 4099 at 4200, 16 / 4 heads x 128, take
-// 365 to 376 us, 0.85 PFLOP/s.  What that cost to reach: half of the score operands read ahead of their products, the products' waves given precedence and V's next
+// 345 to 377 us (by the card's clock), 0.84 to 0.92 PFLOP/s, the matrix unit busy 0.47 of its cycles.  What that cost to reach: half of the score operands read ahead of their products, the products' waves given precedence and V's next
 // fragments read ahead (437 -> 414 us); a copy of a whole tile in a path of its own, so that it is eight instructions and their addresses (404 -> 374); a row's
 // visible keys in bits of a register, not in 64 scalar registers that pushed the loop's own ones out (4 x 1000 at 1000, 12 heads x 64: 59 -> 54).
 template <int HD>
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
 // the 256 registers that the vector unit reaches (with 4 waves for 512 columns the compiler kept O in the others and moved it to and fro: 8 us a tile).
 // The scores of tile i + 1 are made between the same two barriers as the softmax and the products with V of tile i, so that neither unit waits for the other.
 // Maximum and sum of a row are kept by every wave that has a part of it, as in the kernel for few rows, and follow as in the one for many.
-//   Chunks of 192 at 800, 4 heads x 512, take 65 us, 180 TFLOP/s: neither the bytes (44 us with the copies alone) nor the products (14 % of the matrix unit's cycles)
+//   Chunks of 192 at 800, 4 heads x 512, take 65 us, 180 TFLOP/s: neither the bytes (44 us with the copies alone) nor the products (10 % of the matrix unit's cycles)
 // but a wave's own chain through a tile, 430 instructions and four trips to LDS of which the other wave of its SIMD hides a part, and workgroups that fill a CU alone.
 template <int HD, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a) {
