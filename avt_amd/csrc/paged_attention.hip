@@ -828,7 +828,8 @@ Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, i
   // And where rows are few and keys many, four times that, so that streams of different lengths even out, but no fewer than 1024 keys each (with many rows the
   // partial results and the join are as much as the keys: 403 against 440 us without it, chunks of 4099 at 4200).
   const long want = c.bm == 128 ? 3l * cu_count / 2 : 2l * cu_count;
-  const long most = c.bm == 64 ? max_kv / 512 : (max_kv + c.cmin - 1) / c.cmin, one = max_kv < 192 ? 1 : std::min(cu_count / items, (max_kv + 127) / 128);
+  const bool few = max_kv < 192;                               // (keys: two splits of 64 to 96 save less than the join costs)
+  const long most = few ? 1 : c.bm == 64 ? max_kv / 512 : (max_kv + c.cmin - 1) / c.cmin, one = few ? 1 : std::min(cu_count / items, (max_kv + 127) / 128);
   long fill = std::min((want + items - 1) / items, most);
   if (c.bm > 16 && one > fill) { fill = one; c.cmin = 128; }
   const long even = c.bm == 16 ? std::min((8l * cu_count + items - 1) / items, max_kv / 1024) : 0;
@@ -872,8 +873,8 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   AVT_CHECK(q && kcache && vcache && table && cu && kv_lens && out, "avt_paged_attn_fwd: null argument");
   AVT_CHECK(ldq >= (long)H * head_dim && ldo >= (long)H * head_dim && ldq % 8 == 0 && ldo % 8 == 0 && aligned16(q) && aligned16(kcache) && aligned16(vcache) && aligned16(out),
             "avt_paged_attn_fwd: 16-byte aligned rows required");
-  AVT_CHECK(ldq < (1l << 29), "avt_paged_attn_fwd: rows of q are too far apart (%ld)", ldq);
   AVT_CHECK((long)Hkv * head_dim < (1l << 26), "avt_paged_attn_fwd: a token's row is too long (%d heads of %d)", Hkv, head_dim);
+  AVT_CHECK(ldq < (1l << 29), "avt_paged_attn_fwd: rows of q are too far apart (%ld)", ldq);
   AVT_CHECK((long)T * H < 0x7f000000l, "avt_paged_attn_fwd: too many rows for one call (%d tokens of %d heads)", T, H);
   const Choice c = choose(T, R, H, Hkv, head_dim, max_new, max_kv > 0 ? max_kv : 0x7fffffff, CUS);
   AVT_CHECK(c.tiles * Hkv < 0x7f000000l, "avt_paged_attn_fwd: too many rows for one call (%d tokens of %d streams)", T, R);

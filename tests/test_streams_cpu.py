@@ -46,7 +46,8 @@ def attn(**kw):
 
 @pytest.mark.parametrize('kw,match', [(dict(q=None), 'null'), (dict(kv=None), 'null'), (dict(out=None), 'null'), (dict(H=3), 'sizes'), (dict(Hkv=0), 'sizes'), (dict(R=0), 'sizes'), (dict(T=-1), 'sizes'),
                                       (dict(hd=12), 'head_dim'), (dict(hd=0), 'head_dim'), (dict(hd=1032), 'head_dim'), (dict(page=40), 'page'), (dict(ldt=2), 'table'), (dict(width=0), 'table'),
-                                      (dict(npages=-1), 'table'), (dict(ldq=504), '16-byte'), (dict(ldo=508), '16-byte'), (dict(kc=P + 4), '16-byte'), (dict(Hkv=1 << 20, H=1 << 20, ldq=1 << 30, ldo=1 << 30), 'too long'),
+                                      (dict(npages=-1), 'table'), (dict(ldq=504), '16-byte'), (dict(ldo=508), '16-byte'), (dict(kc=P + 4), '16-byte'), (dict(Hkv=1 << 20, H=1 << 20, ldq=1 << 30, ldo=1 << 30), 'too long'), (dict(ldq=1 << 29), 'too far'),
+                                      (dict(width=1 << 21, ldt=1 << 21, page=1024), 'table'),
                                       (dict(T=1 << 29, H=8, ldq=1024, ldo=1024), 'too many'), (dict(ws=None, max_kv=100000, width=8192, ldt=8192), 'workspace'),
                                       (dict(wsb=16, max_kv=100000, width=8192, ldt=8192), 'workspace')])
 def test_attention_refusals(kw, match):
