@@ -743,7 +743,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a)
   }
 }
 
-// The partial results of the splits that a row's keys reach, joined in the splits' order with weights 2^(m_z - max m) in fp32.
+// The partial results of the splits that a row's keys reach, joined in the splits' order with weights 2^(m_z - max m) in fp32.  A weight of 0 does not take a split out:
+// the maximum of a split whose scores are all NaN is -inf (a maximum passes over NaN), and 0 NaN is the NaN that the row has without splits.
 // What both kernels need of a row: how many splits its keys reach.
 __device__ __forceinline__ int splits_of(const AttnArgs& a, int t, int lane) {
   const int r = __builtin_amdgcn_readfirstlane(find_stream(a.cu, a.R, t, lane));
@@ -769,7 +770,8 @@ __global__ __launch_bounds__(256) void paged_attn_join_few_kernel(AttnArgs a) {
   for (int z = 0; z < nz; ++z) {
     const float f = __builtin_amdgcn_exp2f(a.part_ml[(rid + z * step) * 2] - mx), lz = a.part_ml[(rid + z * step) * 2 + 1];
     const f32x4_t p = *(const f32x4_t*)(a.part_o + (rid + z * step) * a.hd + (idx * 4 - h * a.hd));
-    if (f != 0.f) { o += p * f; l += lz * f; }
+    o += p * f;
+    l += lz * f;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *(u32x2_t*)(a.out + (size_t)t * a.ldo + idx * 4) = (u32x2_t){pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)};
@@ -788,7 +790,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
   if (mx == -INFINITY) mx = 0.f;
   for (int z = lane; z < nz; z += 64) {
     const float f = __builtin_amdgcn_exp2f(a.part_ml[(rid + z * step) * 2] - mx);
-    l += f == 0.f ? 0.f : f * a.part_ml[(rid + z * step) * 2 + 1];
+    l += f * a.part_ml[(rid + z * step) * 2 + 1];
     if (tid < 64) wt[z] = f;
   }
   l = wave_sum(l);
@@ -798,8 +800,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
   if (grp < groups)
     for (int z = grp; z < nz; z += groups) {
       const float f = wt[z];
-      const f32x4_t p = *(const f32x4_t*)(a.part_o + (rid + z * step) * a.hd + c * 4);
-      if (f != 0.f) o += p * f;
+      o += *(const f32x4_t*)(a.part_o + (rid + z * step) * a.hd + c * 4) * f;
     }
   sum[tid] = o;
   __syncthreads();

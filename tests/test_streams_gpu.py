@@ -624,3 +624,60 @@ def test_streams_go_past_the_contiguous_cache_kernels_limits(ops):
     parts = torch.cat([a.append(x[i:i + 100], [100]) for i in range(0, 600, 100)])
     close(parts, b.append(x, [600]))
     close(a.rollout(5), b.rollout(5))
+
+
+# A row that sees a NaN has one, however the keys are split.  The hints give one split, a few (joined by the kernel of few splits) and many:
+SPLIT_HINTS = [(100, 1), (250, 4), (1000, 10 ** 9)]             # (max_kv, the most splits it may give)
+
+
+def splits_given(T, R, H, Hkv, hd, max_kv):
+    """Partial results are hd + 2 floats a row and split, behind 16 bytes."""
+    from avt_amd import lib
+    return max(1, (lib.load().avt_paged_attn_workspace_bytes(T, R, H, Hkv, hd, 0, max_kv) - 16) // (4 * T * H * (hd + 2)))
+
+
+@pytest.mark.parametrize('H,Hkv,hd', [(4, 4, 512), (8, 2, 128), (12, 12, 64), (4, 1, 256), (2, 2, 1024)])
+@pytest.mark.parametrize('new', [1, 40])
+@pytest.mark.parametrize('what', ['query', 'keys', 'value'])
+def test_what_is_not_finite_and_seen_stays_however_the_keys_are_split(ops, H, Hkv, hd, new, what):
+    """A query row with one NaN; 256 keys that are all NaN, whole splits of them; an infinite value among 256 keys whose probabilities are 0 in 32 bits (the sum of the
+    definition is infinite): not finite in exactly those rows (for the value: that column), whatever max_kv says; every other row and column as the definition has it."""
+    kv = 1000
+    q, kc, vc, table, cu, kv_lens = make_attn([new, new], [kv, kv - 7], H, Hkv, hd, 16, 7 * hd + new)
+    clean = (q.clone(), kc.clone(), vc.clone())
+    T, grp = 2 * new, H // Hkv
+    hit = torch.zeros((T, H, hd), dtype=torch.bool, device='cuda')
+    put = lambda cache, lo, hi, head, col, x: [cache[int(table[0, j // 16]), j % 16, head, col].fill_(x) for j in range(lo, hi)]
+    if what == 'query':
+        q[0, H - 1, 3] = float('nan')
+        hit[0, H - 1] = True
+    elif what == 'keys':
+        put(kc, 256, 512, Hkv - 1, slice(None), float('nan'))
+        hit[:new, (Hkv - 1) * grp:] = True
+    else:
+        # q = 1 and k = -40 in every column: scale q k is -40 sqrt(hd), at most -320, below the others (random, |scale q k| < 20) by far more than 2^-149
+        q[:new, H - 1] = 1.0
+        put(kc, 256, 512, Hkv - 1, slice(None), -40.0)
+        clean = (q.clone(), kc.clone(), vc.clone())
+        put(vc, 300, 301, Hkv - 1, 5, float('inf'))
+        hit[:new, (Hkv - 1) * grp:, 5] = True
+        hit[:new, (Hkv - 1) * grp:H - 1, 5] = False            # (of the other rows with this kv head the probability may or may not be 0: not looked at)
+    ref, tol = attn_in_64(*clean, table, cu, kv_lens, hd ** -0.5)
+    look = ~hit
+    if what == 'value':
+        look[:new, (Hkv - 1) * grp:, 5] = False
+    given = set()
+    for max_kv, most in SPLIT_HINTS:
+        n = splits_given(T, 2, H, Hkv, hd, max_kv)
+        assert n <= most
+        given.add(min(n, 5))
+        out = ops.paged_attn(q, kc, vc, table, i32(cu), i32(kv_lens), max_kv=max_kv)
+        o = out.view(T, H, hd)
+        if what == 'value':
+            assert not bool(torch.isfinite(o[hit]).any()), max_kv
+        else:
+            assert bool(torch.isnan(o[hit]).all()), max_kv
+        ok = look.view(T, H * hd)
+        assert bool(torch.isfinite(out[ok]).all()), max_kv
+        assert float(((out.double() - ref).abs() - tol)[ok].max()) <= 0, max_kv
+    assert 1 in given and len(given) > 1
