@@ -493,8 +493,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
     }
     __builtin_amdgcn_s_setprio(1);
     const uint32_t va = vaddr0 + stage * 2 * TILEB, vb = va ^ 32;       // rows + 8: the swizzle differs by two pieces
-    // (a tile of which one row sees a key that another one does not: a value that is not finite must not reach the latter through its probability of 0)
-    const bool uneven = first < last && j0 + BN - 1 > first;
+    // (a tile that holds a key which some row of this wave does not see -- the wave's rows may be one token's, the tile's keys reach the workgroup's last one: a value
+    // that is not finite must not reach that row through its probability of 0)
+    const bool uneven = min(j0 + BN, w.k1) - 1 > first;
     bf16x8_t vbuf[2][4];                                       // (the fragments of the next columns are read while these are multiplied)
     const auto read_v = [&](int d) {
       const uint32_t x = va ^ (d * 64), y = vb ^ (d * 64);

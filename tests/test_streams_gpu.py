@@ -681,3 +681,23 @@ def test_what_is_not_finite_and_seen_stays_however_the_keys_are_split(ops, H, Hk
         assert bool(torch.isfinite(out[ok]).all()), max_kv
         assert float(((out.double() - ref).abs() - tol)[ok].max()) <= 0, max_kv
     assert 1 in given and len(given) > 1
+
+
+@pytest.mark.parametrize('H,Hkv,hd', [(32, 1, 128), (64, 2, 64), (48, 1, 128), (64, 1, 40), (40, 1, 256), (32, 1, 512)])
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')])
+def test_many_query_heads_a_kv_head_and_what_a_row_does_not_see(ops, H, Hkv, hd, bad):
+    """32 and more query heads share a kv head, so that all 32 rows of a wave may be one token's: the tile still holds keys of later tokens, for the other waves.  The
+    last tokens' values (two of them, so that rows before, between and at them are there) are not finite: rows that do not see them are as if they were not there."""
+    new, kv = [4, 70, 3, 33], [20, 100, 64, 300]
+    q, kc, vc, table, cu, kv_lens = make_attn(new, kv, H, Hkv, hd, 16, 19)
+    for r, k in enumerate(kv):
+        for j in (k - 1, k - 2):
+            vc[int(table[r, j // 16]), j % 16] = bad
+    ref, tol = attn_in_64(q, kc, torch.nan_to_num(vc, 0, 0, 0), table, cu, kv_lens, hd ** -0.5)
+    for kw in ({}, dict(max_new=70, max_kv=300), dict(max_new=1, max_kv=300)):
+        out = ops.paged_attn(q, kc, vc, table, i32(cu), i32(kv_lens), **kw)
+        for r in range(len(new)):
+            lo, hi = cu[r], cu[r + 1] - 2
+            assert bool(torch.isfinite(out[lo:hi]).all()), (r, kw)
+            assert float(((out[lo:hi].double() - ref[lo:hi]).abs() - tol[lo:hi]).max()) <= 0
+            assert not bool(torch.isfinite(out[hi:cu[r + 1]]).any())                # and what IS seen is passed on
