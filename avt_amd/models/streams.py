@@ -79,14 +79,11 @@ class HeadStreams:
             raise ValueError(f'{-free} pages short: release streams, or open more pages')
         return owned, free
 
-    def _plan(self, lens, counts, host_lens):
-        owned, free = self._take(host_lens, counts)
+    def _plan(self, lens, counts, owned, n_free):
+        """A plan from (lens, owned, n_free) on the device, for counts that _take has let through.  It writes new entries into the table behind the owned ones and
+        nothing else: the pages are taken when the caller keeps the plan's owned and n_free, and free as before if it does not."""
         new = torch.tensor(counts, dtype=torch.int32).to(self.lens.device)
-        plan = ops.paged_plan(lens, new, self.owned, self.table, self.free, self.n_free, self.page, sum(counts))
-        self.owned.copy_(plan.owned)
-        self.n_free.copy_(plan.n_free)
-        self._owned, self._n_free = owned, free
-        return plan
+        return ops.paged_plan(lens, new, owned, self.table, self.free, n_free, self.page, sum(counts))
 
     def _linear(self, layer, name, lin, x, **kw):
         if self._w4 is not None:
@@ -125,7 +122,11 @@ class HeadStreams:
             return feats.new_zeros((0, feats.size(1)), dtype=torch.float32)
         arena = get_arena(self.head)
         arena.refresh_shadow()
-        plan = self._plan(self.lens, counts, self._lens)
+        owned, free = self._take(self._lens, counts)
+        plan = self._plan(self.lens, counts, self.owned, self.n_free)
+        self.owned.copy_(plan.owned)
+        self.n_free.copy_(plan.n_free)
+        self._owned, self._n_free = owned, free
         enc = ops.linear_fwd(feats.to(torch.bfloat16).contiguous(), arena.sh(self.head.encoder.weight))
         hidden = self._blocks(enc, plan, counts, self._lens)
         who = [s for s, c in enumerate(counts) if c]
@@ -138,7 +139,8 @@ class HeadStreams:
     @torch.no_grad()
     def rollout(self, steps):
         """(S, steps, C) fp32: entry 0 is decoded from the hidden state behind each stream's newest frame, entry i from the state reached by feeding the states back
-        i times.  The streams keep their frames only; streams without frames give zeros."""
+        i times.  The streams keep their frames only, and the pool has its pages back afterwards (it has to hold those of the steps while they run); streams without
+        frames give zeros."""
         if steps < 1:
             raise ValueError('rollout: at least one step')
         arena = get_arena(self.head)
@@ -150,13 +152,14 @@ class HeadStreams:
         rows = torch.tensor(live, device=self.last.device)
         counts = [int(l > 0) for l in self._lens]
         self._take(self._lens, [c * (steps - 1) for c in counts])      # (all steps, or none)
-        hidden, lens, host = self.last.index_select(0, rows), self.lens, list(self._lens)
+        hidden, host = self.last.index_select(0, rows), list(self._lens)
+        lens, owned, n_free = self.lens, self.owned, self.n_free       # (followed from step to step and not kept: the pages are the pool's again afterwards)
         for i in range(steps):
             out[rows, i] = self._decode(hidden)
             if i + 1 < steps:
-                plan = self._plan(lens, counts, host)
+                plan = self._plan(lens, counts, owned, n_free)
                 hidden = self._blocks(hidden, plan, counts, host)
-                lens, host = plan.kv_lens, [l + c for l, c in zip(host, counts)]
+                lens, owned, n_free, host = plan.kv_lens, plan.owned, plan.n_free, [l + c for l, c in zip(host, counts)]
         return out
 
     def release(self, which):

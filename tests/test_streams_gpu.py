@@ -701,3 +701,31 @@ def test_many_query_heads_a_kv_head_and_what_a_row_does_not_see(ops, H, Hkv, hd,
             assert bool(torch.isfinite(out[lo:hi]).all()), (r, kw)
             assert float(((out[lo:hi].double() - ref[lo:hi]).abs() - tol[lo:hi]).max()) <= 0
             assert not bool(torch.isfinite(out[hi:cu[r + 1]]).any())                # and what IS seen is passed on
+
+
+@pytest.mark.parametrize('bits', [16, 4])
+def test_a_rollout_keeps_no_page(ops, bits):
+    """A pool that holds the frames and little more: what a roll-out took on its way is free again, and another stream may have it."""
+    head, orc = build_head(64, 64, 2, 2)
+    st = head.open_streams(3, max_len=40, page=8, pages=6, weight_bits=bits)
+    x = torch.randn((48, 64), generator=torch.Generator().manual_seed(8))
+    st.append(x[:15].cuda(), [8, 7, 0])                        # 1 + 1 pages: 4 free
+    state = lambda: (st.lens.tolist(), st.owned.tolist(), int(st.n_free), list(st._owned), st._n_free)
+    before = state()
+    assert before[2] == 4
+    a = st.rollout(12)                                         # 11 frames behind each: 2 pages of stream 0, 2 of stream 1
+    assert state() == before
+    assert torch.equal(a, st.rollout(12)) and state() == before
+    with pytest.raises(ValueError, match='pages short'):
+        st.rollout(20)                                         # 3 + 3 pages: 4 are there
+    assert state() == before
+    out = st.append(x[15:47].cuda(), [0, 0, 32])               # all four free pages
+    assert st.lengths == [8, 7, 32] and int(st.n_free) == 0
+    if bits == 16:
+        close(out, oracle_decode(orc, x[15:47], 1))
+        close(a[0, :4], oracle_decode(orc, x[:8], 4)[7:])
+    b = st.rollout(1)              # (a step more would need a page of stream 0)
+    assert torch.equal(b[:2], a[:2, :1])
+    out = st.append(x[47:48].cuda(), [0, 1, 0])                # stream 1's own page has a row left, which the roll-outs wrote over
+    if bits == 16:
+        close(out, oracle_decode(orc, torch.cat([x[8:15], x[47:48]]), 1)[7:])
