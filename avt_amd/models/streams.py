@@ -120,21 +120,25 @@ class HeadStreams:
             raise ValueError(f'append: ({sum(counts)}, {self.head.in_features}) features for {self.S} counts, got {tuple(feats.shape)} for {len(counts)}')
         if not any(counts):
             return feats.new_zeros((0, feats.size(1)), dtype=torch.float32)
+        if feats.device != self.lens.device:
+            raise ValueError(f'append: features on device {feats.device}, streams on {self.lens.device}')
         arena = get_arena(self.head)
         arena.refresh_shadow()
         owned, free = self._take(self._lens, counts)
         plan = self._plan(self.lens, counts, self.owned, self.n_free)
-        self.owned.copy_(plan.owned)
-        self.n_free.copy_(plan.n_free)
-        self._owned, self._n_free = owned, free
         enc = ops.linear_fwd(feats.to(torch.bfloat16).contiguous(), arena.sh(self.head.encoder.weight))
         hidden = self._blocks(enc, plan, counts, self._lens)
         who = [s for s, c in enumerate(counts) if c]
         ends = torch.tensor([sum(counts[:s + 1]) - 1 for s in who], device=feats.device)
-        self.last.index_copy_(0, torch.tensor(who, device=feats.device), hidden.index_select(0, ends))
+        decoded, last = self._decode(hidden), hidden.index_select(0, ends)
+        who = torch.tensor(who, device=feats.device)
+        # (kept only now: an error on the way here leaves the streams as they were)
+        self.last.index_copy_(0, who, last)
         self.lens.copy_(plan.kv_lens)
-        self._lens = [l + c for l, c in zip(self._lens, counts)]
-        return self._decode(hidden)
+        self.owned.copy_(plan.owned)
+        self.n_free.copy_(plan.n_free)
+        self._lens, self._owned, self._n_free = [l + c for l, c in zip(self._lens, counts)], owned, free
+        return decoded
 
     @torch.no_grad()
     def rollout(self, steps):

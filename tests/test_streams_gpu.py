@@ -729,3 +729,35 @@ def test_a_rollout_keeps_no_page(ops, bits):
     out = st.append(x[47:48].cuda(), [0, 1, 0])                # stream 1's own page has a row left, which the roll-outs wrote over
     if bits == 16:
         close(out, oracle_decode(orc, torch.cat([x[8:15], x[47:48]]), 1)[7:])
+
+
+def test_an_append_that_fails_leaves_the_streams_as_they_were(ops, monkeypatch):
+    """Features on another device, and an error on the way through the blocks: no page is taken, and the same frames may come again."""
+    head, orc = build_head(64, 64, 2, 2)
+    st = head.open_streams(2, max_len=40, page=8, pages=4)
+    x = torch.randn((30, 64), generator=torch.Generator().manual_seed(9))
+    st.append(x[:5].cuda(), [5, 0])
+    state = lambda: (st.lens.tolist(), st.owned.tolist(), int(st.n_free), list(st._owned), st._n_free, st.lengths)
+    before = state()
+    with pytest.raises(ValueError, match='device'):
+        st.append(x[5:25], [20, 0])
+    assert state() == before
+    with monkeypatch.context() as m:
+        calls = []
+
+        def broken(*a, **kw):
+            calls.append(1)
+            if len(calls) > 2:
+                raise RuntimeError('out of memory')
+            return ops_ln(*a, **kw)
+        ops_ln = ops.layernorm_fwd
+        m.setattr(ops, 'layernorm_fwd', broken)
+        with pytest.raises(RuntimeError, match='out of memory'):
+            st.append(x[5:25].cuda(), [20, 0])
+        calls.clear()
+        with pytest.raises(RuntimeError, match='out of memory'):
+            st.rollout(9)
+    assert state() == before
+    out = st.append(x[5:29].cuda(), [3, 21])                   # three pages for stream 1: all four are in use
+    close(out[:3], oracle_decode(orc, x[:8], 1)[5:])
+    close(out[3:], oracle_decode(orc, x[8:29], 1))
