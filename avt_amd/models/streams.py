@@ -35,6 +35,12 @@ class HeadStreams:
         self.pages = self.S * self.width if pages is None else int(pages)
         if self.pages < 1:
             raise ValueError('open_streams: at least one page')
+        if self.S > 4096:
+            raise ValueError(f'open_streams: at most 4096 streams (got {streams})')
+        if self.pages * self.page > 1 << 31:
+            raise ValueError(f'open_streams: a pool of at most 2^31 rows (got {self.pages} pages of {self.page})')
+        if head.inter_dim // head.n_head > 1024:
+            raise ValueError(f'open_streams: heads of at most 1024 columns (got {head.inter_dim // head.n_head})')
         dev = head.encoder.weight.device
         arena = get_arena(head)                                # (raises off the GPU: there is no CPU path)
         E, H = head.inter_dim, head.n_head

@@ -123,3 +123,15 @@ def test_w4_layout_and_rounding():
         assert bool(((p.dequantize() - w).abs() <= s * (0.5 + 7 * 2.0 ** -8) * (1 + 2.0 ** -20)).all())
     with pytest.raises(AvtHipError):
         ops.W4Weight.quantize(w, 48)
+
+
+def test_open_streams_refuses_what_its_operators_would():
+    """Before anything is allocated: more streams than a plan takes, heads wider than the attention's, a pool whose rows no slot could name."""
+    from helpers import build_hip_model
+    head = build_hip_model('feat', 64, 64, 1, 2, 11, device='cpu').future_predictor
+    for kw, match in ((dict(streams=4097), '4096'), (dict(streams=2, pages=1 << 28, page=16), '2\\^31'), (dict(streams=0), 'at least one'), (dict(streams=1, page=12), 'page')):
+        with pytest.raises(ValueError, match=match):
+            head.open_streams(**kw)
+    wide = build_hip_model('feat', 64, 1032, 1, 1, 11, device='cpu').future_predictor
+    with pytest.raises(ValueError, match='1024'):
+        wide.open_streams(2)
