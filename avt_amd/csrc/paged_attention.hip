@@ -871,6 +871,7 @@ extern "C" int avt_paged_attn_fwd(const void* q, long ldq, const void* kcache, c
   AVT_CHECK(head_dim >= 8 && head_dim % 8 == 0 && head_dim <= HDMAX, "avt_paged_attn_fwd: head_dim must be a multiple of 8 in [8, %d] (got %d)", HDMAX, head_dim);
   AVT_CHECK(page >= 8 && page <= 1024 && (page & (page - 1)) == 0, "avt_paged_attn_fwd: the page must be a power of two in [8, 1024] (got %d)", page);
   AVT_CHECK(npages >= 0 && width >= 1 && ldt >= width && (long)width * page < 0x7fff0000l, "avt_paged_attn_fwd: bad table (width %d, ldt %d, page %d)", width, ldt, page);
+  AVT_CHECK(npages <= (1l << 31) / page, "avt_paged_attn_fwd: a cache may hold 2^31 rows, as many as slots name (%ld pages of %d)", npages, page);
   if (T == 0) return 0;
   AVT_CHECK(q && kcache && vcache && table && cu && kv_lens && out, "avt_paged_attn_fwd: null argument");
   AVT_CHECK(ldq >= (long)H * head_dim && ldo >= (long)H * head_dim && ldq % 8 == 0 && ldo % 8 == 0 && aligned16(q) && aligned16(kcache) && aligned16(vcache) && aligned16(out),

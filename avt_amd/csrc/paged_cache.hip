@@ -171,6 +171,7 @@ extern "C" int avt_paged_kv_write(const void* k, long ldk, const void* v, long l
   AVT_CHECK(k && v && kcache && vcache && slots && nslots >= 0, "avt_paged_kv_write: null argument");
   AVT_CHECK(ldk >= width && ldv >= width && ldk % 8 == 0 && ldv % 8 == 0 && aligned16(k) && aligned16(v) && aligned16(kcache) && aligned16(vcache),
             "avt_paged_kv_write: 16-byte aligned rows required");
+  AVT_CHECK(nslots <= 1l << 31, "avt_paged_kv_write: a cache may hold 2^31 rows, as many as slots name (got %ld)", nslots);
   const long total = (long)T * (width / 8);
   AVT_CHECK(total < 0x7f000000l, "avt_paged_kv_write: too many values for one call (%ld rows of %d)", (long)T, width);
   const int blocks = (int)((total + 255) / 256 < 8192 ? (total + 255) / 256 : 8192);

@@ -328,7 +328,8 @@ int avt_sgd_step_dev(float* param, float* grad, float* momentum_buf, void* shado
 /* ---- many streams on one paged key / value cache (ABI 10) ---------------------------------------------------------------
  * What `past_key_values` is to one batch of clips of one length (models/future_prediction.py:168-202), for streams of different lengths that grow by
  * chunks: a pool of pages of `page` tokens (a power of two in [8, 1024]), kcache / vcache bf16 [npages][page][Hkv][head_dim], and per stream a row of
- * `width` page numbers in `table` (int32, row stride ldt; width * page < 2^31 - 2^16).  All int32 arrays live on the device, so a step can be captured and replayed.
+ * `width` page numbers in `table` (int32, row stride ldt; width * page < 2^31 - 2^16).  npages * page <= 2^31: a row of the pool is named by an int32.
+ * All int32 arrays live on the device, so a step can be captured and replayed.
  * avt_paged_plan: R <= 4096 streams of lens[r] cached tokens that own owned[r] pages each take fresh[r] >= 0 new tokens, packed one stream behind the
  *   other into T token rows; free_pages[0 .. *n_free) (at most nfree_max) is a stack of free pages.
  *     cu [R + 1]      first token row of each stream (running sum of fresh);  rows behind cu[R]: slot, position and stream -1

@@ -135,3 +135,15 @@ def test_open_streams_refuses_what_its_operators_would():
     wide = build_hip_model('feat', 64, 1032, 1, 1, 11, device='cpu').future_predictor
     with pytest.raises(ValueError, match='1024'):
         wide.open_streams(2)
+
+
+def test_caches_of_more_rows_than_a_slot_can_name_are_refused():
+    """A slot is an int32: the plan gives rows behind 2^31 - 1 none, so an attention that saw them would see keys that were never written."""
+    with pytest.raises(AvtHipError, match='2\\^31'):
+        attn(npages=(1 << 27) + 1, page=16)
+    with pytest.raises(AvtHipError, match='2\\^31'):
+        attn(npages=1 << 60, page=1024)
+    attn(T=0, q=None, npages=1 << 27, page=16)
+    with pytest.raises(AvtHipError, match='2\\^31'):
+        write(nslots=(1 << 31) + 1)
+    write(T=0, k=None, nslots=1 << 31)
