@@ -147,3 +147,24 @@ def test_caches_of_more_rows_than_a_slot_can_name_are_refused():
     with pytest.raises(AvtHipError, match='2\\^31'):
         write(nslots=(1 << 31) + 1)
     write(T=0, k=None, nslots=1 << 31)
+
+
+@pytest.mark.parametrize('M,N,K,group', [(3, 40, 8192, 64), (4, 96, 10944, 64), (2, 40, 10944, 32)])
+def test_exact_sums_tell_every_mistake(M, N, K, group):
+    """The inputs of the GPU's test of equality, with mistakes planted in the sums: a group left out, first, last or between, a neighbour's scale, weights
+    rounded to bf16, a piece of 32 k left out.  Each moves most outputs (a sum of whole numbers is 0 by chance once in some ten)."""
+    import test_streams_gpu as t
+    x, q, c, _, _, total = t.w4_exact_case(M, N, K, group, M + N + K)
+    u = torch.stack([q & 15, q >> 4], dim=-1).view(N, K).double() - 8
+    s = c.double().repeat_interleave(group, 1)
+    xs, full = x.double(), total.double()
+    assert torch.equal(xs @ (u * s).t(), full)
+    moved = lambda y: float((y != full).double().mean())
+    for lo, n in ((0, group), (K - group, group), (K // 2 // group * group, group), (K // 2 // 32 * 32, 32)):
+        xz = xs.clone()
+        xz[:, lo:lo + n] = 0
+        assert moved(xz @ (u * s).t()) > 0.8
+    s2 = s.clone()
+    s2[:, -group:] = s[:, -2 * group:-group]
+    assert moved(xs @ (u * s2).t()) > 0.8
+    assert moved(xs @ (u * s).to(torch.bfloat16).double().t()) > 0.9

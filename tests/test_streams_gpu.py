@@ -761,3 +761,49 @@ def test_an_append_that_fails_leaves_the_streams_as_they_were(ops, monkeypatch):
     out = st.append(x[5:29].cuda(), [3, 21])                   # three pages for stream 1: all four are in use
     close(out[:3], oracle_decode(orc, x[:8], 1)[5:])
     close(out[3:], oracle_decode(orc, x[8:29], 1))
+
+
+# ---- 4-bit linear: sums that are exact --------------------------------------------------------------------------------------------------------
+def w4_exact_case(M, N, K, group, seed):
+    """Inputs whose every partial sum, in any order, is a whole number of 2^-7 below 2^24 of them, i.e. exact in fp32: x in -2 .. 2, scales of 8 significant bits
+    c 2^-7 with odd c in 129 .. 255 (a weight (u - 8) s has up to 11 bits and would not survive a rounding to bf16), bias and residual whole numbers.
+    Returns CPU tensors (x, q bytes, scales, bias, res, exact) with exact int64 in units of 2^-7."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-2, 3, (M, K), generator=g)
+    q = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8)
+    c = 2 * torch.randint(64, 128, (N, K // group), generator=g) + 1
+    bias, res = torch.randint(-9, 10, (N,), generator=g), torch.randint(-9, 10, (M, N), generator=g)
+    total, bound = torch.zeros((M, N), dtype=torch.int64), torch.zeros((M, N), dtype=torch.int64)
+    for i in range(K // group):                                # (products of whole numbers in fp64: exact)
+        b = q[:, i * group // 2:(i + 1) * group // 2]
+        xs, us = x[:, i * group:(i + 1) * group].double(), torch.stack([b & 15, b >> 4], dim=-1).view(N, group).double()
+        part = (xs @ (us - 8).t()).long() * c[:, i]
+        total += part
+        bound += part.abs()
+        assert int((xs.abs() @ (us + 16).t()).max()) < 1 << 24                       # inside a group: products of 16 + u, and 24 sum x
+    assert int(bound.max()) + 9 * 128 * 2 < 1 << 24
+    return x, q, c, bias, res, total
+
+
+def w4_case_on_gpu(ops, x, q, c, bias, res):
+    K = x.size(1)
+    wide = torch.zeros((x.size(0), K + 8), device='cuda', dtype=BF16)
+    wide[:, :K] = x.cuda()
+    return wide[:, :K], ops.W4Weight(q.cuda(), (c.cuda().double() / 128).to(BF16)), bias.float().cuda(), res.cuda().to(BF16)
+
+
+W4_EXACT = [(1, 2048, 2048, 128), (3, 100, 8192, 64), (7, 15, 8192, 128), (4, 96, 10944, 64), (2, 17, 96, 32), (16, 64, 192, 64), (17, 33, 256, 128), (33, 1000, 544, 32),
+            (64, 2048, 2048, 64), (64, 48, 8192, 32), (36, 12300, 1376, 32), (48, 6200, 4160, 64), (20, 12300, 1152, 128), (33, 12300, 8192, 128), (65, 50, 10944, 32), (200, 130, 8192, 128)]
+
+
+@pytest.mark.parametrize('M,N,K,group', W4_EXACT)
+def test_w4_linear_of_exact_sums_is_exact(ops, M, N, K, group):
+    """Every weight, scale and group counts once, unrounded: equal, in fp32, with and without bias and residual."""
+    x, q, c, bias, res, total = w4_exact_case(M, N, K, group, M + N + K)
+    xd, w, bd, rd = w4_case_on_gpu(ops, x, q, c, bias, res)
+    y = ops.w4_linear(xd, w, out_mode=ops.OUT_F32)
+    assert torch.equal(y.double().cpu() * 128, total.double())
+    y = ops.w4_linear(xd, w, bias=bd, res=rd, out_mode=ops.OUT_F32)
+    assert torch.equal(y.double().cpu() * 128, (total + 128 * (bias + res)).double())
+    y = ops.w4_linear(xd, w)                                   # and rounded once
+    assert torch.equal(y.cpu(), (total.double() / 128).float().to(BF16))
