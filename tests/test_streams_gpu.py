@@ -807,3 +807,20 @@ def test_w4_linear_of_exact_sums_is_exact(ops, M, N, K, group):
     assert torch.equal(y.double().cpu() * 128, (total + 128 * (bias + res)).double())
     y = ops.w4_linear(xd, w)                                   # and rounded once
     assert torch.equal(y.cpu(), (total.double() / 128).float().to(BF16))
+
+
+@pytest.mark.parametrize('counts', [[1] * 64, [90, 0, 200, 1, 37]])
+def test_four_bit_streams_of_many_rows(ops, counts):
+    """64 streams of one frame each, and chunks of hundreds of rows: the same as a head whose projections hold the values that the 4-bit weights stand for."""
+    from avt_amd.models.streams import HeadStreams
+    head, _ = build_head(128, 256, 2, 2)
+    st4 = head.open_streams(len(counts), max_len=300, weight_bits=4)
+    with torch.no_grad():
+        for b in head.gpt_model.h:
+            for lin in (b.attn.c_attn, b.attn.c_proj, b.mlp.c_fc, b.mlp.c_proj):
+                lin.weight.copy_(HeadStreams._quantize(lin.weight).dequantize().t())
+    st = head.open_streams(len(counts), max_len=300)
+    x = torch.randn((2, sum(counts), 128), generator=torch.Generator().manual_seed(5)).cuda()
+    for f in x[:2 if max(counts) < 100 else 1]:
+        close(st4.append(f, counts), st.append(f, counts))
+    close(st4.rollout(2), st.rollout(2))
