@@ -384,7 +384,7 @@ __global__ __launch_bounds__(256) void paged_attn_tile_kernel(AttnArgs a) {
 // for the tile.  The running maximum follows only when a score passes it by more than 2^8: the probabilities then stay below 2^8, where bf16 and the fp32
 // sums are as exact as below 1, and the accumulators are rarely rescaled.
 //   Two workgroups share a CU, two waves a SIMD, of which one's softmax is to run beside the other's products: chunks of 4099 at 4200, 16 / 4 heads x 128, take
-// 345 to 377 us (by the card's clock), 0.84 to 0.92 PFLOP/s, the matrix unit busy 0.47 of its cycles.  What that cost to reach: half of the score operands read ahead of their products, the products' waves given precedence and V's next
+// 362 us among other launches, 372 alone in a graph, 384 under the profiler, 0.83 to 0.88 PFLOP/s, the matrix unit busy 0.46 of its cycles there.  What that cost to reach: half of the score operands read ahead of their products, the products' waves given precedence and V's next
 // fragments read ahead (437 -> 414 us); a copy of a whole tile in a path of its own, so that it is eight instructions and their addresses (404 -> 374); a row's
 // visible keys in bits of a register, not in 64 scalar registers that pushed the loop's own ones out (4 x 1000 at 1000, 12 heads x 64: 59 -> 54).
 template <int HD>
@@ -554,8 +554,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_long_kernel(AttnArgs a) {
 // the 256 registers that the vector unit reaches (with 4 waves for 512 columns the compiler kept O in the others and moved it to and fro: 8 us a tile).
 // The scores of tile i + 1 are made between the same two barriers as the softmax and the products with V of tile i, so that neither unit waits for the other.
 // Maximum and sum of a row are kept by every wave that has a part of it, as in the kernel for few rows, and follow as in the one for many.
-//   Chunks of 192 at 800, 4 heads x 512, take 65 us, 180 TFLOP/s: neither the bytes (44 us with the copies alone) nor the products (10 % of the matrix unit's cycles)
-// but a wave's own chain through a tile, 430 instructions and four trips to LDS of which the other wave of its SIMD hides a part, and workgroups that fill a CU alone.
+//   16 chunks of up to 192 at up to 800, 4 heads x 512, take 66 us, 175 TFLOP/s: the longest workgroup has 31 tiles of 2.1 us, where an even share would be 13.3 a CU (180
+// workgroups on 256 CUs, of 9 to 31 tiles; 16 chunks that all are the longest take the same, 69 us).  11 x 976 at 42, 8 / 2 heads x 512, are even, 52 tiles a CU, and take 157 us and
+// not 110: with one workgroup on a CU nothing runs beside finding the work, fetching Q and the first tiles, and the stores.  Inside a tile it is a wave's own chain, 430
+// instructions and four trips to LDS, of which the other wave of its SIMD hides a part: the copies alone take 44 us, the products 10 % of the matrix unit's cycles.
 template <int HD, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void paged_attn_wide_kernel(AttnArgs a) {
   constexpr int BN = 32, BM = 64, ROWB = HD * 2, TILEB = BN * ROWB, DS = HD / 32, KB = 8 / NW, DT = HD / 128, NB = 8 / NW;      // KB: key blocks of a wave's S, NB: row blocks of its O
@@ -825,12 +827,17 @@ Choice choose(int T, int R, int H, int Hkv, int hd, long max_new, long max_kv, i
   const long items = c.tiles * Hkv;
   // Enough workgroups for two on every CU (one and a half, where 128 rows each make a split's partial results dear), down to 64 keys each of few rows (a tile of 16
   // to 64 keys is 0.9 us of latency, a join 4: 1 x 730, 8 heads x 128, 14 us in splits of 256 keys, 9.4 in splits of 64), 256 of 128 rows and 512 of 64 rows of a
-  // wide head (chunks of 192 at 800, 4 heads x 512: 71 us whole, 87 in four).  With many rows, only to have one on every CU, down to 128 keys (3 x 680 at 1168, one
-  // head x 128: 24 us in 8, 21 in 15; 32 x 40 at 500, 8 / 2 heads x 128, which has enough: 21 us in splits of 256 keys, 25 in splits of 128).
+  // wide head (4 heads x 512, 16 chunks of 192 at 800: 67 us whole, 80 in splits of 256 keys, 95 against 69 where all are the longest; 20 x 20 at 3000: 91 in splits of 512,
+  // 101 of 256, 176 whole; 8 heads x 256, 8 x 300 at 2000: 111, 112, 125).  With many rows, only to have one on every CU, down to 128 keys (3 x 680 at 1168, one
+  // head x 128: 24 us in 8, 21 in 15; 32 x 40 at 500, 8 / 2 heads x 128, which has enough: 21 us in splits of 256 keys, 25 in splits of 128; 4 x 200 at 600, 8 heads x 512:
+  // 43, 54 without).
   // And where rows are few and keys many, four times that, so that streams of different lengths even out, but no fewer than 1024 keys each (with many rows the
   // partial results and the join are as much as the keys: 403 against 440 us without it, chunks of 4099 at 4200).
   const long want = c.bm == 128 ? 3l * cu_count / 2 : 2l * cu_count;
-  const bool few = max_kv < 192;                               // (keys: two splits of 64 to 96 save less than the join costs)
+  // No splits below 192 keys.  One new token each, in a graph, whole and in splits of 64: 12 heads x 64, 3 x 1 at 150 7.0 and 9.0 us; 8 / 2 heads x 128, 16 x 1 at 150 8.3 and
+  // 9.5, 1 x 1 at 190 9.0 and 8.7.  The rule is that of tiles of 32 and 64 keys; heads whose tiles are 16 keys pay for it where streams are few: 4 heads x 256, 3 x 1 at 150 13.5
+  // and 11.6 us, 64 x 1 at 150 15.5 and 17.2; 4 heads x 512, 3 x 1 at 100 14.0 and 12.9, at 190 20.5 and 13.8, 64 x 1 at 190 25.0 and 25.4; 2 heads x 1024, 3 x 1 at 190 29.4 and 18.0.
+  const bool few = max_kv < 192;
   const long most = few ? 1 : c.bm == 64 ? max_kv / 512 : (max_kv + c.cmin - 1) / c.cmin, one = few ? 1 : std::min(cu_count / items, (max_kv + 127) / 128);
   long fill = std::min((want + items - 1) / items, most);
   if (c.bm > 16 && one > fill) { fill = one; c.cmin = 128; }

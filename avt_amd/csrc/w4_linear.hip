@@ -41,7 +41,7 @@ __device__ __forceinline__ void copy_to_lds(const void* base, char* lds, uint32_
 // the waves.  Products are of the exact integers 16 + u with the bf16 x, in fp32, and begin at -24 sum x, a product with a matrix of -24, so a group ends with
 // y += s sum: the weights are never rounded.
 //   1 x 2048 x 2048 3.3 us, 3 x 2048 x 8192 7.8 us, both the launch and one round of loads; 1 x 16384 x 8192 16.1 us, 4.3 TB/s of weights and scales; 33 rows of
-// the same 27.5 us: 18.8 without the products, whose operands (weights unpacked, x paired, a wave's 3 x 4 tiles in 250 registers) leave two waves a SIMD.
+// the same 25.1 us among launches on other inputs, 28 to 30 alone: 18.8 of 27.5 without the products, whose operands (weights unpacked, x paired, a wave's 3 x 4 tiles in 250 registers) leave two waves a SIMD.
 //   A load whose neighbouring lanes read different rows takes the vector cache 4 cycles per 64 bytes (measured: 59 cycles for 64 x 16 bytes of 16 rows, and these
 // loads, not the bytes, set the time: 43 us of 33 x 16384 x 8192 against 24 without those of x), but that is how the matrix unit wants its operands.  So neighbouring
 // lanes fetch neighbouring bytes -- weights 64 bytes of each of 16 rows, copied straight into LDS, x 256 bytes of each of 4 rows, through registers -- and a wave
@@ -222,6 +222,11 @@ int launch(const W4Args& a, hipStream_t st) {
   return 0;
 }
 // (A last tile of at most 4 rows asks for those only: 33 rows of 16384 x 8192 27.9 us, 29.1 with the whole tile; of 2048 x 8192 13.9, 15.1.)
+// 33 to 48 rows take three tiles of 16 rows at once and read the weights once; in two blocks of two tiles 33 rows of 6144 x 2048 take 11.6 us instead of 8.0, 48 of 16384 x 8192 44
+// instead of 32.7, but 48 of 2048 x 8192 12.5 instead of 16 (one tile of columns each: half of the CUs idle, and two blocks fill them).  From 49 rows on there are two blocks either
+// way, and two tiles are the faster up to 64 (64 rows of 16384 x 8192 47.3 us, 55.8 with three); three would be from 65 to 96 (96 rows 67.9, 58.3), and of 6144 x 2048 beyond (1000
+// rows 144, 113).  The weights are unpacked again for every block of rows, so that from about 100 rows on (of 2048 x 8192, from about 300) the bf16 product of the unpacked weight is faster: 64
+// rows of 6144 x 2048 14.4 us here and 15.2 there, 256 rows 42 and 23, 3000 rows 410 and 102.
 template <int NT, int GS>
 int launch_cols(const W4Args& a, hipStream_t st) {
   if (a.M <= 4) return launch<1, NT, GS, 1>(a, st);
@@ -232,6 +237,9 @@ int launch_cols(const W4Args& a, hipStream_t st) {
   if (a.M > 32 && a.M <= 48) return launch<3, NT3, GS, 4>(a, st);
   return launch<2, NT, GS, 4>(a, st);
 }
+// As many columns a workgroup as leave three of every four CUs one (more columns share what x costs, fewer workgroups leave CUs idle).  With one / two / four tiles of 16 columns:
+// 1 row of 2048 x 8192 6.9 / 9.0 / 12.5 us, of 6144 x 2048 4.9 / 4.4 / 6.4, of 12288 x 2048 7.3 / 7.4 / 7.0; 33 rows of 2048 x 8192 13.6 / 16.9 / 23.9,
+// of 6144 x 2048 11.9 / 7.8 / 12.2, of 12288 x 2048 20.1 / 16.9 / 12.6, of 16384 x 8192 52.6 / 37.0 / 29.1.
 template <int GS>
 int launch_rows(const W4Args& a, hipStream_t st) {
   return a.N >= 64 * 192 ? launch_cols<4, GS>(a, st) : a.N >= 32 * 192 ? launch_cols<2, GS>(a, st) : launch_cols<1, GS>(a, st);

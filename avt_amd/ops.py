@@ -796,7 +796,8 @@ def _paged_attn_workspace(*dims):
 def paged_attn(q, kcache, vcache, table, cu, kv_lens, *, scale=None, max_new=0, max_kv=0, out=None):
     """Causal attention of each stream's new tokens (rows cu[r] .. cu[r + 1) of q [T, H, head_dim]) over its kv_lens[r] cached tokens, the new ones among them
     (avt_paged_attn_fwd) -> [T, H * head_dim].  A chunk of one token is a decode step.  max_new / max_kv: the longest chunk and the longest kv_lens, as far as the caller
-    knows them (they choose kernels, not results).  Rows behind cu[R] are not written."""
+    knows them (they choose kernels, not results).  Rows behind cu[R] are not written.  Scores, maxima and sums are fp32; probabilities are rounded to bf16, the matrix unit's
+    type, for the product with v (causal_attn_decode keeps them in fp32)."""
     P, page, Hkv, hd = _cache_dims(kcache, vcache)
     ldq = _token_rows(q, 'q')
     T, H, hq = q.shape
@@ -853,7 +854,8 @@ class W4Weight:
 
 
 def w4_linear(x, w, *, bias=None, act=ACT_NONE, res=None, out_mode=OUT_BF16, out=None):
-    """y[M, N] = epilogue(x[M, K] @ w^T) for a W4Weight (avt_w4_linear): + bias, tanh GELU, + res as in gemm(); made for few rows, where the weights' bytes count."""
+    """y[M, N] = epilogue(x[M, K] @ w^T) for a W4Weight (avt_w4_linear): + bias, tanh GELU, + res as in gemm(); made for few rows, where the weights' bytes count: the
+    weights are unpacked again for every block of rows, and from about 100 rows on the bf16 product of ``w.dequantize()`` is faster."""
     N, K = w.N, w.K
     if x.dim() != 2 or x.dtype != BF16 or x.size(1) != K or x.stride(1) != 1:
         _refuse(f'x must be bf16 [M, {K}] with unit inner stride, got {tuple(x.shape)} {x.dtype}')

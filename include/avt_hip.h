@@ -343,6 +343,8 @@ int avt_sgd_step_dev(float* param, float* grad, float* momentum_buf, void* shado
  * avt_paged_attn_fwd: q [T][H][head_dim] (token stride ldq), out [T][H * head_dim] (row stride ldo): rows cu[r] .. cu[r + 1) are the n newest of stream r's
  *   kv_lens[r] cached tokens; row i of them sits at x = kv_lens[r] - n + i and out = softmax(scale q k[0..x]^T) v[0..x] with the kv head h / (H / Hkv); 0 where
  *   no key is seen.  Keys a row does not see have no influence on it, whatever their bits.  A table entry outside [0, npages) names no page: its keys are not seen.
+ *   However the keys are split, a NaN that is seen makes its rows NaN (in v: that column of them) and an infinite value that column not finite; a score of -inf is a
+ *   probability of 0, and a row that has no other is 0.  Probabilities are rounded to bf16 for the product with v.
  *   Rows behind cu[R] are left as they are.  head_dim % 8 == 0, <= 1024.  max_new / max_kv: what the caller knows of the longest chunk and of the longest
  *   kv_lens (0: nothing); they choose kernels and grids, results hold for any lengths.  ws: avt_paged_attn_workspace_bytes of the same arguments.
  * avt_w4_linear: y[m, n] = epilogue(sum_k x[m, k] s[n, k / group] (u[n, k] - 8)): x bf16 [M][K], u in 0 .. 15 two to a byte (q [N][K / 2], the low nibble holds
