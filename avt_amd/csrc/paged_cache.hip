@@ -151,6 +151,7 @@ extern "C" int avt_paged_plan(const int* lens, const int* fresh, const int* owne
   AVT_CHECK(T == 0 || (slots && positions && streams), "avt_paged_plan: null token output");
   AVT_CHECK(R >= 1 && R <= PLAN_RMAX, "avt_paged_plan: 1 to %d streams (got %d)", PLAN_RMAX, R);
   AVT_CHECK(T >= 0 && nfree_max >= 0 && width >= 1 && ldt >= width, "avt_paged_plan: bad sizes (T %d, free %d, width %d, ldt %d)", T, nfree_max, width, ldt);
+  AVT_CHECK(T < 0x7ff00000, "avt_paged_plan: fewer than 2^31 - 2^20 token rows (got %d)", T);      // (a thread's row and the grid's stride stay an int)
   AVT_CHECK(page >= 8 && page <= 1024 && (page & (page - 1)) == 0, "avt_paged_plan: the page must be a power of two in [8, 1024] (got %d)", page);
   AVT_CHECK((long)width * page < 0x7fff0000l, "avt_paged_plan: a stream may hold fewer than 2^31 - 2^16 tokens (width %d, page %d)", width, page);
   const int blocks = T <= PLAN_NT ? 1 : (T + PLAN_NT - 1) / PLAN_NT < 512 ? (T + PLAN_NT - 1) / PLAN_NT : 512, lds = (4 * R + 1) * 4;

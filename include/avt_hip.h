@@ -331,7 +331,7 @@ int avt_sgd_step_dev(float* param, float* grad, float* momentum_buf, void* shado
  * `width` page numbers in `table` (int32, row stride ldt; width * page < 2^31 - 2^16).  npages * page <= 2^31: a row of the pool is named by an int32.
  * All int32 arrays live on the device, so a step can be captured and replayed.
  * avt_paged_plan: R <= 4096 streams of lens[r] cached tokens that own owned[r] pages each take fresh[r] >= 0 new tokens, packed one stream behind the
- *   other into T token rows; free_pages[0 .. *n_free) (at most nfree_max) is a stack of free pages.
+ *   other into T < 2^31 - 2^20 token rows; free_pages[0 .. *n_free) (at most nfree_max) is a stack of free pages.
  *     cu [R + 1]      first token row of each stream (running sum of fresh);  rows behind cu[R]: slot, position and stream -1
  *     pages           stream r needs max(0, ceil((lens + fresh) / page) - owned) more, popped off the stack in the order of the streams and written behind
  *                     the table's owned[r] entries.  A stream is refused when its pages pass `width`, its token rows pass T, or the stack does not hold what it and

@@ -168,3 +168,10 @@ def test_exact_sums_tell_every_mistake(M, N, K, group):
     s2[:, -group:] = s[:, -2 * group:-group]
     assert moved(xs @ (u * s2).t()) > 0.8
     assert moved(xs @ (u * s).to(torch.bfloat16).double().t()) > 0.9
+
+
+def test_plan_refuses_rows_that_its_threads_could_not_count():
+    """A thread goes on by up to 512 x 1024 rows: from 2^31 - 2^20 rows on that could pass 2^31 and come out negative."""
+    for T in (2 ** 31 - 1, 2 ** 31 - 2 ** 19, 2 ** 31 - 2 ** 20):
+        with pytest.raises(AvtHipError, match='2\\^31 - 2\\^20'):
+            plan(T=T)
