@@ -58,6 +58,11 @@ def flops_skipped_per_clip(D, T, S=197):
     return 3 * T * (full - done)
 
 
+def four_digits(x):
+    """Four significant digits: a slow step's fraction (0.00091, and 0.00087 of it executed) is still one."""
+    return float(f'{x:.4g}')
+
+
 def algorithmic_bytes_per_step(D, L, T, B, Dh=2048, Lh=6, S=197, folded=None):
     """HBM bytes per step per GPU of the implemented dataflow if every tensor crossed HBM exactly as often as the kernel
     sequence consumes / produces it (DESIGN.md section 4 lists the per-kernel terms).  Unit u = one [tokens, D] bf16 tensor.
@@ -329,8 +334,8 @@ def main(argv=None):
         D, L, _ = VIT[a.model]
         fclip = flops_per_clip(D, L, a.frames)
         step_tf = clips_per_s / world * fclip / 1e12
-        out = {'achieved': round(step_tf, 1), 'frac': round(step_tf / MFMA_PEAK_TFLOPS, 4),
-               'executed_frac': round(clips_per_s / world * (fclip - flops_skipped_per_clip(D, a.frames)) / 1e12 / MFMA_PEAK_TFLOPS, 4)}
+        out = {'achieved': round(step_tf, 1), 'frac': four_digits(step_tf / MFMA_PEAK_TFLOPS),
+               'executed_frac': four_digits(clips_per_s / world * (fclip - flops_skipped_per_clip(D, a.frames)) / 1e12 / MFMA_PEAK_TFLOPS)}
         if tr:
             rows = [r for r in gemm_rows(tr, steps, step_s) if r['kernel'].startswith(BIG)]
             fl = sum(r['tflops'] * r['ms_per_step'] for r in rows)            # TFLOP/s x ms = GFLOP per step
@@ -369,7 +374,7 @@ def main(argv=None):
         rl = roofline_of(args, clips, trace, tsteps, tstep_s)
         roof = {'bound': 'mfma', 'scope': 'whole training step (fwd + bwd + SGD) per GPU: clips/s/GPU x algorithmic GFLOP/clip (SURVEY 8d)',
                 'achieved': round(step_tf, 1), 'peak': MFMA_PEAK_TFLOPS, 'unit': 'TFLOP/s',
-                'frac': round(step_tf / MFMA_PEAK_TFLOPS, 4),
+                'frac': four_digits(step_tf / MFMA_PEAK_TFLOPS),
                 'frac_counts': 'algorithmic FLOPs (SURVEY 8d), including the part of the last ViT block that the CLS-only evaluation skips',
                 'executed_frac': rl['executed_frac'],
                 'traffic': None if pmc is None else pmc['hbm_bytes_per_step'],

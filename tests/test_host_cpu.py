@@ -576,3 +576,12 @@ def test_zeroed_gradient_registry_against_a_brute_force_model():
     los, his = ops._ZEROED[base][1]
     assert los == sorted(los) and all(h <= l for h, l in zip(his[:-1], los[1:]))
     ops.forget_zeroed()
+
+
+def test_bench_fractions_keep_four_digits_however_slow_the_step():
+    """The executed part of a step is smaller than the whole also where both are below a thousandth of the peak."""
+    import bench
+    assert bench.four_digits(0.38424) == 0.3842 and bench.four_digits(0.000914351) == 0.0009144 and bench.four_digits(0.0) == 0.0
+    whole, skipped = bench.flops_per_clip(768, 12, 10), bench.flops_skipped_per_clip(768, 10)
+    for clips in (0.5, 2.5, 975.2):
+        assert bench.four_digits(clips * (whole - skipped) / 1e12 / 2500) < bench.four_digits(clips * whole / 1e12 / 2500)
